@@ -130,7 +130,8 @@ def _plain_lce(x, w, b, labels, in_out, need_grad):
     at = torch.where(valid, labels, torch.zeros_like(labels)).long()[:, None]
     picked = logits.gather(1, at)
     loss = torch.where(valid, (lse - picked)[:, 0], torch.zeros_like(lse[:, 0])).sum() / count
-    out = dict(loss=loss, lse=lse[:, 0])
+    # a row without a label is not evaluated: its log-sum-exp is given as 0
+    out = dict(loss=loss, lse=torch.where(valid, lse[:, 0], torch.zeros_like(lse[:, 0])))
     if not need_grad:
         return out
     d = logits.sub_(lse).exp_()
@@ -223,7 +224,7 @@ def _exact_lce(s):
     rows = torch.nonzero(labels != IGNORE)[:, 0]
     n_valid = max(1, rows.numel())
     loss = (lse[rows] - z[rows, labels[rows]]).sum() / n_valid
-    out = dict(loss=loss, lse=lse)
+    out = dict(loss=loss, lse=torch.zeros_like(lse).index_copy(0, rows, lse[rows]))
     if c["grad"]:
         p = torch.zeros_like(z)
         p[rows] = torch.exp(z[rows] - lse[rows, None]) / n_valid
