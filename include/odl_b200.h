@@ -186,6 +186,21 @@ int odl_softmax_cross_entropy(const float *logits, const void *labels, int label
 int odl_softmax_cross_entropy_static(const float *logits, const void *labels, int labels_are_int64, int64_t B, int64_t C,
                                      float *loss, float *dlogits, float grad_scale, void *stream);
 
+/* Loss of a linear head over many classes, with its gradients, without handing out the logits:
+ *   z = x[M,K] . op(W) + b;  lse[i] = log sum_j exp z[i,j];  loss[0] = (1/n) sum_i (lse[i] - z[i,t_i]), i over the n rows
+ *   whose label is not ignore_index;  dx, dw, db: the gradients of grad_scale * loss (dw in the layout of w).
+ * Stands for Linear (w_layout as in odl_linear_forward) followed by SoftmaxCrossEntropy
+ * (src/operators/loss/softmax_cross_entropy.cpp:17-111) and their backward passes; the loss is the log-sum-exp form,
+ * without the 1e-8 inside the reference's logarithm.
+ * A row whose label is ignore_index takes no part: lse = 0, dx = 0, and whatever its x holds reaches no output; with no row
+ * left the loss and the gradients are 0.  A label outside [0, N) other than ignore_index is reported by odl_device_status
+ * (ODL_ERR_INVALID_ARGUMENT) and its row treated like an ignored one.  A bias of -infinity takes a class out.
+ * b, loss, lse[M], dx[M,K], dw, db[N] may each be NULL; at least one output is required.  Scratch comes from the arena; calls
+ * on different streams are ordered behind one another. */
+int odl_linear_cross_entropy(const float *x, const float *w, const float *b, const void *labels, int labels_are_int64,
+                             int64_t ignore_index, int64_t M, int64_t N, int64_t K, int w_layout, float *loss, float *lse,
+                             float *dx, float *dw, float *db, float grad_scale, int precision, void *stream);
+
 /* ---- optimizers -------------------------------------------------------------------------------------------------- */
 
 /* One fused in-place Adam update of n contiguous parameters at step t (1-based), same operation order and fp32 rounding
@@ -200,6 +215,23 @@ int odl_adam_step(float *param, float *grad, float *m, float *v, float *param_sm
  * after the optional WeightDecay hook.  momentum_buf may be NULL when momentum == 0. */
 int odl_sgd_step(float *param, float *grad, float *momentum_buf, float *param_small, int64_t n, float lr, float momentum,
                  float weight_decay, int nesterov, float hook_weight_decay, float grad_scale, void *stream);
+
+/* out = the Newton-Schulz orthogonalisation of each of `batch` matrices g[rows, cols]: X = g / max(|g|_F, eps), then
+ * `steps` times X = 3.4445 X + (-4.7750 A + 2.0315 A^2) X with A = X X^T (the smaller side's Gram matrix), which takes the
+ * singular values of X towards 1 (0.7 .. 1.2 after five steps).  out may be g.  No counterpart in the reference. */
+int odl_newton_schulz(const float *g, float *out, int64_t batch, int64_t rows, int64_t cols, int steps, float eps, int precision,
+                      void *stream);
+
+/* One fused in-place Muon update of `batch` equal-shaped weight matrices [rows, cols] (contiguous, one behind the other):
+ *   g = grad * grad_scale + hook_weight_decay * param (written back to grad when it differs, as in odl_sgd_step);
+ *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  U = newton_schulz(u, steps, eps);
+ *   param = param * (1 - lr * weight_decay) - lr * sqrt(max(1, fan_out / fan_in)) * U.
+ * w_layout says which side is fan_out (ODL_W_OUT_IN: rows).  momentum_buf may be NULL when momentum == 0.  param_small:
+ * optional output, low part of the updated parameters for the next 3xTF32 GEMM.  No counterpart in the reference, whose
+ * optimizers are SGD and Adam. */
+int odl_muon_step(float *param, float *grad, float *momentum_buf, float *param_small, int64_t batch, int64_t rows, int64_t cols,
+                  int w_layout, float lr, float momentum, float weight_decay, int nesterov, float hook_weight_decay,
+                  float grad_scale, int steps, float eps, int precision, void *stream);
 
 /* ---- Conv2d (im2col + GEMM) -------------------------------------------------------------------------------------- */
 

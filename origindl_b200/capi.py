@@ -66,6 +66,10 @@ _SIGNATURES = {
     "odl_softmax_cross_entropy": [_P, _P, c_int, _I64, _I64, _P, _P, c_float, _P],
     "odl_adam_step": [_P, _P, _P, _P, _P, _I64, c_int, c_float, c_float, c_float, c_float, c_float, c_float, _P],
     "odl_sgd_step": [_P, _P, _P, _P, _I64, c_float, c_float, c_float, c_int, c_float, c_float, _P],
+    "odl_linear_cross_entropy": [_P, _P, _P, _P, c_int, _I64, _I64, _I64, _I64, c_int, _P, _P, _P, _P, _P, c_float, c_int, _P],
+    "odl_newton_schulz": [_P, _P, _I64, _I64, _I64, c_int, c_float, c_int, _P],
+    "odl_muon_step": [_P, _P, _P, _P, _I64, _I64, _I64, c_int, c_float, c_float, c_float, c_int, c_float, c_float, c_int,
+                      c_float, c_int, _P],
     "odl_im2col": [_P, _P, _I64, _I64, _I64, _I64, c_int, c_int, c_int, c_int, _P],
     "odl_col2im": [_P, _P, _I64, _I64, _I64, _I64, c_int, c_int, c_int, c_int, _P],
     "odl_conv2d_forward": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, c_int, c_int, c_int, c_int, c_int, c_int, _P],

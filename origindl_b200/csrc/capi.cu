@@ -26,6 +26,8 @@ struct DeviceState
     char *arena     = nullptr;
     size_t capacity = 0;
     size_t used     = 0;
+    bool recorded   = false;          // a graph holds addresses inside the block (arena_begin during capture)
+    cudaEvent_t last_use = nullptr;   // behind the last call that ended with arena_end
 };
 DeviceState g_state;
 std::mutex g_mu;
@@ -89,9 +91,10 @@ void *arena_alloc(size_t bytes)
         }
         if (cudaDeviceSynchronize() != cudaSuccess)
             return nullptr;
-        if (g_state.arena)
-            cudaFree(g_state.arena);
+        if (g_state.arena && !g_state.recorded)
+            cudaFree(g_state.arena);  // (a recorded block stays: the graph that holds it may be replayed)
         g_state.arena    = nullptr;
+        g_state.recorded = false;
         g_state.capacity = 0;
         size_t want      = bytes + (bytes >> 2);
         void *p          = nullptr;
@@ -120,6 +123,56 @@ int arena_reserve(size_t total_bytes)
     if (!p)
         return kCudaError;
     g_state.used = 0;
+    return kOk;
+}
+
+int arena_begin(size_t bytes, cudaStream_t stream)
+{
+    int dev = -1;
+    ODL_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev != g_state.device)
+    {
+        set_last_error("the current device is %d, odl_init bound device %d", dev, g_state.device);
+        return kInvalidArgument;
+    }
+    arena_reset();
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess)
+    {
+        cudaGetLastError();  // the default stream while another one is captured: the launches will report it
+        capture = cudaStreamCaptureStatusNone;
+    }
+    if (capture != cudaStreamCaptureStatusNone)
+    {
+        if (bytes + 4096 > g_state.capacity)
+        {
+            set_last_error("scratch arena: %zu bytes needed while a graph is being captured, %zu held: make the same call once "
+                           "before the capture",
+                           bytes + 4096, g_state.capacity);
+            return kNotInitialized;
+        }
+        g_state.recorded = true;
+        return kOk;
+    }
+    int rc = arena_reserve(bytes);
+    if (rc)
+        return rc;
+    if (g_state.last_use)
+        ODL_CUDA_TRY(cudaStreamWaitEvent(stream, g_state.last_use, 0));
+    return kOk;
+}
+
+int arena_end(cudaStream_t stream)
+{
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone)
+    {
+        cudaGetLastError();
+        return kOk;  // inside a graph the order is the graph's own
+    }
+    if (!g_state.last_use)
+        ODL_CUDA_TRY(cudaEventCreateWithFlags(&g_state.last_use, cudaEventDisableTiming));
+    ODL_CUDA_TRY(cudaEventRecord(g_state.last_use, stream));
     return kOk;
 }
 
@@ -346,6 +399,11 @@ int odl_device_status(void *stream)
         if (flag == 3)
         {
             set_last_error("gather_rows: sample index out of range");
+            return kInvalidArgument;
+        }
+        if (flag == 4)
+        {
+            set_last_error("linear_cross_entropy: label out of range");
             return kInvalidArgument;
         }
         gemm_pair_recover(s);  // a persistent GEMM that gave up may have left its unit counters mid-launch

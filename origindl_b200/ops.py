@@ -157,6 +157,40 @@ def softmax_cross_entropy(logits, labels, need_grad=True, grad_scale=1.0):
     return loss.reshape(()), d
 
 
+def _same_device(*tensors):
+    for t in tensors:
+        if t is not None and t.get_device() != torch.cuda.current_device():
+            raise ValueError(f"odl ops need tensors on the current device, got one on {t.device}")
+
+
+def linear_cross_entropy(x, w, labels, b=None, ignore_index=-100, need_dx=True, need_dw=True, need_db=None, grad_scale=1.0,
+                         w_layout=W_OUT_IN, precision=PRECISION_3XTF32):
+    """Softmax cross entropy of the head x @ op(w) (+ b) without its logits: (loss 0-dim, lse (M,), dx, dw, db), all on the
+    device; a gradient that is not asked for is None and is not computed (need_db defaults to `b is not None`).  The loss is
+    the mean over the rows whose label is not ignore_index; ignored rows have lse = 0 and dx = 0."""
+    _chk(x, w, b)
+    if labels.dtype not in (torch.int32, torch.int64) or not labels.is_cuda or not labels.is_contiguous():
+        raise TypeError("labels must be a contiguous int32/int64 CUDA tensor")
+    _same_device(x, w, b, labels)
+    if x.dim() != 2 or w.dim() != 2 or labels.dim() != 1 or labels.shape[0] != x.shape[0]:
+        raise ValueError("linear_cross_entropy expects x (M, K), a 2-D weight and labels (M,)")
+    M, K = x.shape
+    N, Kw = w.shape if w_layout == W_OUT_IN else (w.shape[1], w.shape[0])
+    if K != Kw:
+        raise ValueError(f"linear_cross_entropy: input features {K} do not match weight {tuple(w.shape)}")
+    if b is not None and tuple(b.shape) != (N,):
+        raise ValueError("linear_cross_entropy: bias size mismatch")
+    need_db = b is not None if need_db is None else need_db
+    loss = torch.empty((1,), device=x.device, dtype=torch.float32)
+    lse = torch.empty((M,), device=x.device, dtype=torch.float32)
+    dx = torch.empty_like(x) if need_dx else None
+    dw = torch.empty_like(w) if need_dw else None
+    db = torch.empty((N,), device=x.device, dtype=torch.float32) if need_db else None
+    capi.call("odl_linear_cross_entropy", _p(x), _p(w), _p(b), labels.data_ptr(), int(labels.dtype == torch.int64),
+              int(ignore_index), M, N, K, w_layout, _p(loss), _p(lse), _p(dx), _p(dw), _p(db), float(grad_scale), precision, _s())
+    return loss.reshape(()), lse, dx, dw, db
+
+
 def adam_step(p, g, m, v, t, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, hook_weight_decay=0.0, grad_scale=1.0,
               p_small=None):
     _chk(p, g, m, v, p_small)
@@ -169,6 +203,38 @@ def sgd_step(p, g, buf=None, lr=1e-2, momentum=0.0, weight_decay=0.0, nesterov=F
     _chk(p, g, buf, p_small)
     capi.call("odl_sgd_step", _p(p), _p(g), _p(buf), _p(p_small), p.numel(), lr, momentum, weight_decay, int(nesterov),
               hook_weight_decay, grad_scale, _s())
+
+
+def _matrices(t, what):
+    if t.dim() not in (2, 3):
+        raise ValueError(f"{what}: expected a matrix (rows, cols) or a stack (batch, rows, cols), got {tuple(t.shape)}")
+    return (1, *t.shape) if t.dim() == 2 else tuple(t.shape)
+
+
+def newton_schulz(g, steps=5, eps=1e-7, precision=PRECISION_3XTF32, out=None):
+    """Newton-Schulz orthogonalisation of g (rows, cols), or of each matrix of a stack (batch, rows, cols)."""
+    _chk(g, out)
+    _same_device(g, out)
+    batch, rows, cols = _matrices(g, "newton_schulz")
+    out = torch.empty_like(g) if out is None else out
+    if out.shape != g.shape:
+        raise ValueError("newton_schulz: out must have the shape of g")
+    capi.call("odl_newton_schulz", _p(g), _p(out), batch, rows, cols, int(steps), float(eps), precision, _s())
+    return out
+
+
+def muon_step(p, g, buf=None, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, hook_weight_decay=0.0, grad_scale=1.0,
+              steps=5, eps=1e-7, w_layout=W_OUT_IN, precision=PRECISION_3XTF32, p_small=None):
+    """One in-place Muon update of a weight matrix, or of a stack of equal-shaped ones (batch, rows, cols)."""
+    _chk(p, g, buf, p_small)
+    _same_device(p, g, buf, p_small)
+    batch, rows, cols = _matrices(p, "muon_step")
+    for t in (g, buf, p_small):
+        if t is not None and t.shape != p.shape:
+            raise ValueError(f"muon_step: a buffer of shape {tuple(t.shape)} does not match the parameter {tuple(p.shape)}")
+    capi.call("odl_muon_step", _p(p), _p(g), _p(buf), _p(p_small), batch, rows, cols, w_layout, float(lr), float(momentum),
+              float(weight_decay), int(nesterov), float(hook_weight_decay), float(grad_scale), int(steps), float(eps), precision,
+              _s())
 
 
 def conv_out_size(size, k, s, p):
