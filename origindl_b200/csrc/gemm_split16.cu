@@ -1,0 +1,219 @@
+// Host side of the split-fp16 GEMM: tensor maps and how many CTAs of a kernel the GPU holds; and the pass that splits a
+// fp32 matrix tile by tile.
+#include "gemm_split16.cuh"
+
+#include "internal.h"
+#include "split16_encode.h"
+
+namespace odl
+{
+namespace s16
+{
+
+int make_tmap_split16(CUtensorMap *out, const Split16 &m, int box_rows)
+{
+    return make_tmap_half3d(out, m.data, 2 * static_cast<int64_t>(m.cols_pad), m.rows, m.batch, m.pitch, m.batch_stride, kBK, box_rows);
+}
+
+int sm_count()
+{
+    static int n = 0;
+    if (n == 0)
+    {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            n = 148;
+    }
+    return n;
+}
+
+// CTAs (cluster == 1) or CTA pairs of `kernel` the device holds at once; 0 with the error text set on failure.
+int resident_ctas(const void *kernel, int cluster, int smem)
+{
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess)
+    {
+        set_last_error("cudaFuncSetAttribute(smem=%d) failed: %s", smem, cudaGetErrorString(e));
+        return 0;
+    }
+    if (cluster == 1)
+        return sm_count();
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim          = dim3(static_cast<unsigned>(sm_count() & ~1), 1, 1);
+    cfg.blockDim         = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id               = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs                = attr;
+    cfg.numAttrs             = 1;
+    int n                    = 0;
+    e                        = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n <= 0)
+    {
+        set_last_error("no CTA pair of the split-fp16 GEMM fits: %s", cudaGetErrorString(e));
+        return 0;
+    }
+    return n;
+}
+
+Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_split, bool sym)
+{
+    (void)terms;
+    struct Kind
+    {
+        int cg, bn;
+        double per_kb, fixed;  // of a tile: a K-block, and filling the ring + storing
+    };
+    const Kind kinds[3] = {{2, 256, 1.0, 4.0}, {1, 128, 0.52, 3.0}, {1, 64, 0.36, 2.5}};
+    const int64_t n_kb  = (K + kBK - 1) / kBK;
+    const double sms    = sm_count();
+    Plan best;
+    double best_t = 1e300;
+    for (const Kind &k : kinds)
+    {
+        const int bm     = 128 * k.cg;
+        if (sym && bm != k.bn)
+            continue;  // (a symmetric output needs square tiles)
+        const int64_t tn = (N + k.bn - 1) / k.bn, tm = (M + bm - 1) / bm;
+        const int64_t tiles = (sym ? tn * (tn + 1) / 2 : tm * tn) * batch;
+        for (int s = 1; s <= (may_split ? 16 : 1); ++s)
+        {
+            const int64_t kb = (n_kb + s - 1) / s;
+            if (s > 1 && kb < 8)
+                break;
+            const double slots = sms / k.cg;
+            const double waves = static_cast<double>((tiles * s + static_cast<int64_t>(slots) - 1) / static_cast<int64_t>(slots));
+            // slices are written and read once more: M N s floats there and back
+            const double t = waves * (k.per_kb * kb + k.fixed) + (s > 1 ? 4.0 + static_cast<double>(M) * N * batch * s * 8 / 7e6 : 0.0);
+            if (t < best_t)
+                best_t = t, best.cg = k.cg, best.bn = k.bn, best.splits = s;
+        }
+    }
+    return best;
+}
+
+namespace
+{
+// One 128 x 64 tile per block: read once, its largest finite value gives the tile's power of two, written as halves.
+// Bound by memory: 4 bytes in and 4 out per value.  TRANSPOSED: element (r, c) is src[c * ld + r].
+template <bool TRANSPOSED>
+__global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restrict__ src, int64_t ld, int rows, int cols, const int *__restrict__ gather,
+                                                            const int *__restrict__ count, __half *__restrict__ out, int64_t pitch,
+                                                            float *__restrict__ scale, bool vec)
+{
+    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 128;
+    const int live = count ? min(rows, *count) : rows;
+    if (r0 >= live)
+        return;  // (gathered matrices: nobody reads rows past the last 128 that hold any)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float2 v[16];
+    if (TRANSPOSED)
+    {
+        __shared__ float tile[64][129];
+        for (int i = warp; i < 64; i += 8)
+        {
+            const float *line = src + (c0 + i) * ld + r0;
+            for (int j = 0; j < 4; ++j)
+            {
+                const int r           = lane + 32 * j;
+                tile[i][r] = (c0 + i < cols && r0 + r < live) ? __ldg(line + r) : 0.f;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = make_float2(tile[2 * lane][warp + 8 * i], tile[2 * lane + 1][warp + 8 * i]);
+    }
+    else
+    {
+        const int c = c0 + 2 * lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            const int r = r0 + warp + 8 * i;
+            v[i]        = make_float2(0.f, 0.f);
+            if (r < live)
+            {
+                const float *line = src + static_cast<int64_t>(gather ? gather[r] : r) * ld;
+                if (vec)
+                {
+                    if (c < cols)
+                        v[i] = __ldg(reinterpret_cast<const float2 *>(line + c));
+                }
+                else
+                {
+                    if (c < cols)
+                        v[i].x = __ldg(line + c);
+                    if (c + 1 < cols)
+                        v[i].y = __ldg(line + c + 1);
+                }
+            }
+        }
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+    {
+        // infinities and NaN stay what they are and choose no scale
+        const float a = fabsf(v[i].x), b = fabsf(v[i].y);
+        top = fmaxf(top, a < INFINITY ? a : 0.f);
+        top = fmaxf(top, b < INFINITY ? b : 0.f);
+    }
+    __shared__ float box[8];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0)
+        box[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+        top = fmaxf(top, box[w]);
+    // s = 2^(e - 14) with 2^e <= top < 2^(e + 1): v / s below 2^15, fp16's largest is just under 2^16
+    const int e     = top > 0.f ? max(ilogbf(top), -112) : 0;
+    const float s   = __int_as_float((e - 14 + 127) << 23);
+    const float inv = __int_as_float((127 - (e - 14)) << 23);
+    if (threadIdx.x == 0)
+        scale[static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y] = s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+    {
+        const int r = r0 + warp + 8 * i;
+        if (r < (gather ? r0 + 128 : rows))
+        {
+            uint32_t hi, lo;
+            split2(v[i].x * inv, v[i].y * inv, hi, lo);
+            uint32_t *line = reinterpret_cast<uint32_t *>(out + r * pitch + 2 * c0);
+            line[lane]      = hi;
+            line[32 + lane] = lo;
+        }
+    }
+}
+}  // namespace
+
+int split16_encode(const float *src, int64_t ld, int transposed, int rows, int cols, const int *gather, const int *count, const Split16 &out,
+                   float *scale, cudaStream_t stream)
+{
+    const dim3 grid((rows + 127) / 128, out.cols_pad / 64);
+    if (grid.y > 65535)
+    {
+        set_last_error("split: %d columns exceed 65535 blocks of 64", cols);
+        return kTooLarge;
+    }
+    const bool vec = !(cols & 1) && !(ld & 1) && !(reinterpret_cast<uintptr_t>(src) & 7);
+    __half *dst    = const_cast<__half *>(out.data);
+    if (transposed)
+        split16_tiles_kernel<true><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, vec);
+    else
+        split16_tiles_kernel<false><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, vec);
+    ++g_launch_count;
+    ODL_CUDA_TRY(cudaGetLastError());
+    return kOk;
+}
+
+}  // namespace s16
+}  // namespace odl

@@ -530,6 +530,31 @@ int make_tmap_mn3d(CUtensorMap *out, const float *ptr, int64_t k_rows, int64_t m
     return r == CUDA_SUCCESS ? kOk : kCudaError;
 }
 
+int make_tmap_half3d(CUtensorMap *out, const void *ptr, int64_t cols, int64_t rows, int64_t batch, int64_t ld, int64_t batch_stride,
+                     int box_cols, int box_rows)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn)
+    {
+        set_last_error("cuTensorMapEncodeTiled entry point not available");
+        return kCudaError;
+    }
+    cuuint64_t dims[3]    = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(batch)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(batch > 1 ? batch_stride : ld * rows) * 2};
+    cuuint32_t box[3]     = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+    cuuint32_t estr[3]    = {1, 1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(ptr), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+    {
+        set_last_error("cuTensorMapEncodeTiled failed: code %d (rows=%lld cols=%lld batch=%lld ld=%lld ptr=%p)", (int)r,
+                       (long long)rows, (long long)cols, (long long)batch, (long long)ld, ptr);
+        return kCudaError;
+    }
+    return kOk;
+}
+
 namespace
 {
 template <int BN, int BK>

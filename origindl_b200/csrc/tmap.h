@@ -18,6 +18,11 @@ int make_tmap(CUtensorMap *out, const float *ptr, int64_t rows, int64_t cols, in
 int make_tmap_mn3d(CUtensorMap *out, const float *ptr, int64_t k_rows, int64_t mn_cols, int64_t ld, int box_k, int boxes,
                    CUtensorMapSwizzle swizzle);
 
+// Tensor map over `batch` row-major matrices of halves, rows x cols each (row pitch ld, matrices batch_stride apart, both in
+// halves), with a {box_cols, box_rows, 1} tile of 128-byte rows, 128-byte swizzle.
+int make_tmap_half3d(CUtensorMap *out, const void *ptr, int64_t cols, int64_t rows, int64_t batch, int64_t ld, int64_t batch_stride,
+                     int box_cols, int box_rows);
+
 struct alignas(64) TmapPack
 {
     CUtensorMap a, a_small, b, b_small;
