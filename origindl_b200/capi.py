@@ -51,6 +51,7 @@ _SIGNATURES = {
     "odl_debug_set_persistent_pairs": [c_int],
     "odl_debug_set_stream_k": [c_int],
     "odl_debug_set_conv_mode": [c_int],
+    "odl_debug_set_loss_piece": [c_int],
     "odl_binary": [c_int, _P, _P, _P, _I64, _P],
     "odl_scale": [_P, c_float, _P, _I64, _P],
     "odl_axpy": [c_float, _P, _P, _I64, _P],

@@ -78,13 +78,15 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_
         const int bm     = 128 * k.cg;
         if (sym && bm != k.bn)
             continue;  // (a symmetric output needs square tiles)
+        if (g_bn_override && (sym && g_bn_override == 64 ? 128 : g_bn_override) != k.bn)
+            continue;
         const int64_t tn = (N + k.bn - 1) / k.bn, tm = (M + bm - 1) / bm;
         const int64_t tiles = (sym ? tn * (tn + 1) / 2 : tm * tn) * batch;
         for (int s = 1; s <= (may_split ? 16 : 1); ++s)
         {
             const int64_t kb = (n_kb + s - 1) / s;
-            if (s > 1 && kb < 8)
-                break;
+            if (may_split && g_split_k > 0 ? s != g_split_k : s > 1 && kb < 8)
+                continue;
             const double slots = sms / k.cg;
             const double waves = static_cast<double>((tiles * s + static_cast<int64_t>(slots) - 1) / static_cast<int64_t>(slots));
             // slices are written and read once more: M N s floats there and back

@@ -430,6 +430,9 @@ int gemm(const s16::Plan &plan, int terms, const Split16 &A, const Split16 &B, c
     return terms == 3 ? s16::launch_plan<3, SCALED, Epi>(plan, A, B, g, ep, stream) : s16::launch_plan<1, SCALED, Epi>(plan, A, B, g, ep, stream);
 }
 
+// Test hook: rows of a piece, a multiple of 256 (0 = from kPieceBytes).
+int g_lce_piece = 0;
+
 inline bool aligned32(const float *p, int64_t ld)
 {
     return !(reinterpret_cast<uintptr_t>(p) & 31) && !(ld & 7);
@@ -474,6 +477,8 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     // rows per piece
     int64_t piece = grads ? kPieceBytes / (static_cast<int64_t>(np) * 4) : 65536;
     piece         = piece < 256 ? 256 : piece / 256 * 256;
+    if (g_lce_piece > 0)
+        piece = g_lce_piece;
     if (piece > m_pad)
         piece = m_pad;
     const int R = static_cast<int>(piece < M ? piece : M);
@@ -592,6 +597,12 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
 }
 
 }  // namespace odl
+
+extern "C" int odl_debug_set_loss_piece(int rows)
+{
+    odl::g_lce_piece = rows > 0 ? (rows + 255) / 256 * 256 : 0;
+    return 0;
+}
 
 extern "C" int odl_linear_cross_entropy(const float *x, const float *w, const float *b, const void *labels, int labels_are_int64,
                                         int64_t ignore_index, int64_t M, int64_t N, int64_t K, int w_layout, float *loss,

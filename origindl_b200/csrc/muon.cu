@@ -1,12 +1,23 @@
 // Orthogonalised updates of weight matrices: the quintic Newton-Schulz iteration and the momentum step around it.
-//   X_0 = u / max(|u|_F, eps);   X <- a X + (b A + c A^2) X,  A = X X^T  (X^T X for tall matrices: the smaller side)
-// with (a, b, c) = (3.4445, -4.7750, 2.0315) drives the singular values of X towards 1.
+//   X_0 = u / max(|u|_F, eps);   X <- S X,  S = a I + b A + c A^2,  A = X X^T
+// (X <- X S with A = X^T X for tall matrices: always the smaller side) with (a, b, c) = (3.4445, -4.7750, 2.0315) drives the
+// singular values of X towards 1.
+//
+// Everything between u and the result is held split-fp16 (gemm_split16.cuh) with ONE power of two per matrix, which the
+// normalisation makes safe: |X|_F <= 1 at first and the singular values stay below 1.21 afterwards, so no entry of X, A or S
+// exceeds 1.21, 1.46 or 3.45; halves scaled by 2^14 (S: 2^13) reach neither the largest fp16 nor, in a way that counts, the
+// smallest: the grid 2^-39 of an entry adds at most 2^-39 sqrt(rows cols) to the Frobenius norm 1 of X, less than the 2^-24 of
+// fp32 itself up to 2^30 entries.  A and S are symmetric: their GEMMs compute the tiles on and above the diagonal and write each
+// twice, which leaves s s l + s^3 + 2 s s l operations a step (s, l the smaller and larger side) of the 2 + 2 + 2.
+// a X is folded into S (a on the diagonal), so a step is three GEMMs and nothing else; the last one's epilogue writes the result
+// or the updated parameters.
 #include <cuda_runtime.h>
 
 #include <cmath>
 
 #include "../../include/odl_b200.h"
-#include "gemm_tc.cuh"
+#include "gemm_epilogue.cuh"
+#include "gemm_split16.cuh"
 #include "host_util.h"
 #include "internal.h"
 
@@ -15,13 +26,25 @@ namespace odl
 
 namespace
 {
+using s16::GemmArgs;
+using s16::Split16;
+using s16::TileAt;
+
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-constexpr int kNormBlocks = 256;
+constexpr float kSx = 16384.f, kSa = 16384.f, kSs = 8192.f;  // halves hold value * this
+constexpr int kNormBlocks = 256;                              // at most, per matrix
 
 inline size_t a256(size_t x)
 {
     return (x + 255) & ~size_t(255);
 }
+
+#define MUON_LAUNCHED()                 \
+    do                                  \
+    {                                   \
+        ++g_launch_count;               \
+        ODL_CUDA_TRY(cudaGetLastError()); \
+    } while (0)
 
 struct MomentumArgs
 {
@@ -29,29 +52,59 @@ struct MomentumArgs
     int nesterov;
 };
 
-// buf = momentum * buf + g, u = nesterov ? g + momentum * buf : buf (the order of the SGD step); squares summed in double
-__global__ void __launch_bounds__(256) muon_momentum_kernel(const float *p, float *g, float *buf, float *u, int64_t n, MomentumArgs a,
-                                                            double *partial)
+// buf = momentum * buf + g, u = nesterov ? g + momentum * buf : buf (operation by operation as in the SGD step)
+__device__ __forceinline__ float momentum_one(float &g, float &buf, float p, bool has_buf, const MomentumArgs &a)
 {
-    double s           = 0;
-    const bool write_g = p && (a.hook_wd > 0.f || a.grad_scale != 1.f);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    if (a.grad_scale != 1.f)
+        g = __fmul_rn(g, a.grad_scale);
+    if (a.hook_wd > 0.f)
+        g = __fadd_rn(g, __fmul_rn(p, a.hook_wd));
+    if (!has_buf)
+        return g;
+    buf = __fadd_rn(__fmul_rn(buf, a.momentum), g);
+    return a.nesterov ? __fadd_rn(g, __fmul_rn(buf, a.momentum)) : buf;
+}
+
+// grid (blocks, batch): momentum in place and the sum of squares of u, in double (no size of gradient over- or underflows)
+__global__ void __launch_bounds__(256) muon_momentum_kernel(const float *__restrict__ p, float *g, float *buf, int64_t n, MomentumArgs a, bool vec,
+                                                            double *__restrict__ partial)
+{
+    const int64_t off  = static_cast<int64_t>(blockIdx.y) * n;
+    const bool write_g = p && (a.hook_wd > 0.f || a.grad_scale != 1.f), read_p = p && a.hook_wd > 0.f;
+    double s = 0;
+    g += off;
+    buf = buf ? buf + off : nullptr;
+    p   = p ? p + off : nullptr;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+    int64_t i            = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (vec)
     {
-        float v = g[i];
-        if (a.grad_scale != 1.f)
-            v = __fmul_rn(v, a.grad_scale);
-        if (p && a.hook_wd > 0.f)
-            v = __fadd_rn(v, __fmul_rn(p[i], a.hook_wd));
-        if (write_g)
-            g[i] = v;
-        if (buf)
+        const int64_t n4 = n >> 2;
+        for (; i < n4; i += stride)
         {
-            const float m = __fadd_rn(__fmul_rn(buf[i], a.momentum), v);
-            buf[i]        = m;
-            v             = a.nesterov ? __fadd_rn(v, __fmul_rn(m, a.momentum)) : m;
+            float4 G = reinterpret_cast<const float4 *>(g)[i];
+            float4 M = buf ? reinterpret_cast<const float4 *>(buf)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 P = read_p ? reinterpret_cast<const float4 *>(p)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float u0 = momentum_one(G.x, M.x, P.x, buf, a), u1 = momentum_one(G.y, M.y, P.y, buf, a);
+            const float u2 = momentum_one(G.z, M.z, P.z, buf, a), u3 = momentum_one(G.w, M.w, P.w, buf, a);
+            if (buf)
+                reinterpret_cast<float4 *>(buf)[i] = M;
+            if (write_g)
+                reinterpret_cast<float4 *>(g)[i] = G;
+            s += static_cast<double>(u0) * u0 + static_cast<double>(u1) * u1;
+            s += static_cast<double>(u2) * u2 + static_cast<double>(u3) * u3;
         }
-        u[i] = v;
-        s += static_cast<double>(v) * v;
+        i = (n4 << 2) + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    }
+    for (; i < n; i += stride)
+    {
+        float G = g[i], M = buf ? buf[i] : 0.f;
+        const float u = momentum_one(G, M, read_p ? p[i] : 0.f, buf, a);
+        if (buf)
+            buf[i] = M;
+        if (write_g)
+            g[i] = G;
+        s += static_cast<double>(u) * u;
     }
     __shared__ double box[8];
     for (int o = 16; o > 0; o >>= 1)
@@ -63,94 +116,349 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const float *p, floa
     {
         for (int w = 1; w < 8; ++w)
             s += box[w];
-        partial[blockIdx.x] = s;
+        partial[blockIdx.y * gridDim.x + blockIdx.x] = s;
     }
 }
 
-__global__ void __launch_bounds__(256) muon_scale_kernel(float *u, int64_t n, const double *partial, float eps)
+// X = u / max(|u|, eps) in halves; u is formed again from g and the updated buf (the same operations, the same bits).
+// grid (blocks, batch); a warp per block of 64 columns of a row.
+__global__ void __launch_bounds__(256) muon_split_kernel(const float *__restrict__ g, const float *__restrict__ buf, int rows, int cols, int cols_pad,
+                                                         float momentum, int nesterov, const double *__restrict__ partial, int n_partial, float eps,
+                                                         __half *__restrict__ x, int64_t x_stride)
 {
-    double s = 0;
-    for (int i = 0; i < kNormBlocks; ++i)
-        s += partial[i];
-    const double norm = sqrt(s);
-    const double inv  = 1.0 / (norm > eps ? norm : static_cast<double>(eps));
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-        u[i] = static_cast<float>(u[i] * inv);
-}
-
-// S = a I + b A + c A^2, in place of A^2
-__global__ void muon_poly_kernel(float *s, const float *a, int m)
-{
-    const int64_t n = static_cast<int64_t>(m) * m;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-        s[i] = kNsC * s[i] + kNsB * a[i] + (i / m == i % m ? kNsA : 0.f);
-}
-
-__global__ void muon_update_kernel(float *p, const float *x, float *p_small, int64_t n, float keep, float rate)
-{
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    __shared__ double box[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double s       = 0;
+    for (int i = threadIdx.x; i < n_partial; i += 256)
+        s += partial[blockIdx.y * n_partial + i];
+    for (int o = 16; o > 0; o >>= 1)
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0)
+        box[warp] = s;
+    __syncthreads();
+    // the factor in double: 1 / norm of a tiny or huge gradient need not be a float
+    double norm = 0;
+    for (int w = 0; w < 8; ++w)
+        norm += box[w];
+    norm             = sqrt(norm);
+    const double inv = static_cast<double>(kSx) / (norm > eps || !(norm == norm) ? norm : static_cast<double>(eps));
+    const int64_t off = static_cast<int64_t>(blockIdx.y) * rows * cols;
+    const int blocks  = cols_pad / 64;
+    const int64_t all = static_cast<int64_t>(rows) * blocks;
+    g += off;
+    buf = buf ? buf + off : nullptr;
+    uint32_t *out = reinterpret_cast<uint32_t *>(x + blockIdx.y * x_stride);
+    for (int64_t k = static_cast<int64_t>(blockIdx.x) * 8 + warp; k < all; k += static_cast<int64_t>(gridDim.x) * 8)
     {
-        const float v = __fsub_rn(__fmul_rn(p[i], keep), __fmul_rn(rate, x[i]));
-        p[i]          = v;
-        if (p_small)
-            p_small[i] = tf32_small(v);
+        const int row = static_cast<int>(k / blocks), c = static_cast<int>(k % blocks) * 64 + 2 * lane;
+        float v[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (c + j < cols)
+            {
+                const int64_t at = static_cast<int64_t>(row) * cols + c + j;
+                const float m    = buf ? buf[at] : 0.f;
+                v[j]             = !buf ? g[at] : nesterov ? __fadd_rn(g[at], __fmul_rn(m, momentum)) : m;
+            }
+        uint32_t hi, lo;
+        s16::split2(static_cast<float>(v[0] * inv), static_cast<float>(v[1] * inv), hi, lo);
+        out[k * 64 + lane]      = hi;
+        out[k * 64 + 32 + lane] = lo;
     }
 }
 
-int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, float *out, float *param, float *param_small,
-                  float keep, float rate, int64_t batch, int64_t rows, int64_t cols, int steps, float eps, int precision,
-                  cudaStream_t stream)
+// ---- epilogues -----------------------------------------------------------------------------------------------------------
+// N columns of this thread's row into a split matrix: 64-column blocks of [hi][lo], 32 bytes a store (whole sectors)
+__device__ __forceinline__ void st_words8(__half *p, const uint32_t (&w)[8])
 {
-    const int64_t n = rows * cols, m = rows < cols ? rows : cols;
-    const bool tall = rows > cols;
-    auto padded     = [&](int64_t r, int64_t c) { return 2 * a256(static_cast<size_t>(r) * ((c + 3) & ~int64_t(3)) * 4); };
-    int rc          = kOk;
-    for (int64_t i = 0; i < batch; ++i)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+template <int NC>
+__device__ __forceinline__ void store_split_row(__half *row, int col, int cols_pad, const float (&v)[NC])
+{
+#pragma unroll
+    for (int i = 0; i < NC; i += 16)
     {
-        if ((rc = arena_begin(2 * a256(n * 4) + 2 * a256(m * m * 4) + a256(kNormBlocks * 8) +
-                                  steps * (4 * padded(rows, cols) + 6 * padded(m, m)),
-                              stream)))
-            return rc;
-        float *x        = static_cast<float *>(arena_alloc(n * 4));
-        float *y        = static_cast<float *>(arena_alloc(n * 4));
-        float *A        = static_cast<float *>(arena_alloc(m * m * 4));
-        float *S        = static_cast<float *>(arena_alloc(m * m * 4));
-        double *partial = static_cast<double *>(arena_alloc(kNormBlocks * 8));
-        muon_momentum_kernel<<<kNormBlocks, 256, 0, stream>>>(p ? p + i * n : nullptr, g + i * n, buf ? buf + i * n : nullptr, x, n, a, partial);
-        muon_scale_kernel<<<592, 256, 0, stream>>>(x, n, partial, eps);
-        g_launch_count += 2;
-        for (int k = 0; k < steps; ++k)
+        const int c = col + i;
+        if (c < cols_pad)
         {
-            rc = tall ? gemm_dispatch(1, 0, m, m, rows, x, nullptr, cols, x, nullptr, cols, A, nullptr, m, nullptr, nullptr, 0, nullptr, 0,
-                                      precision, stream, false)
-                      : gemm_dispatch(0, 1, m, m, cols, x, nullptr, cols, x, nullptr, cols, A, nullptr, m, nullptr, nullptr, 0, nullptr, 0,
-                                      precision, stream, false);
-            if (rc || (rc = gemm_dispatch(0, 0, m, m, m, A, nullptr, m, A, nullptr, m, S, nullptr, m, nullptr, nullptr, 0, nullptr, 0,
-                                          precision, stream, false)))
-                return rc;
-            muon_poly_kernel<<<592, 256, 0, stream>>>(S, A, (int)m);
-            ++g_launch_count;
-            rc = tall ? gemm_dispatch(0, 0, rows, cols, m, x, nullptr, cols, S, nullptr, m, y, nullptr, cols, nullptr, nullptr, 0, nullptr,
-                                      0, precision, stream, false)
-                      : gemm_dispatch(0, 0, rows, cols, m, S, nullptr, m, x, nullptr, cols, y, nullptr, cols, nullptr, nullptr, 0, nullptr,
-                                      0, precision, stream, false);
-            if (rc)
-                return rc;
-            float *t = x;
-            x = y, y = t;
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s16::split2(v[i + 2 * j], v[i + 2 * j + 1], hi[j], lo[j]);
+            __half *p = row + (c >> 6) * 128 + (c & 63);
+            st_words8(p, hi);
+            st_words8(p + 64, lo);
         }
-        if (param)
+    }
+}
+
+// the transpose of a warp's 32 rows x NC columns: row `col + i` of the matrix receives 32 consecutive columns.  Neighbouring
+// lanes swap one of two values, so that a lane holds two neighbouring columns of one row and stores them as a word.
+template <int NC>
+__device__ __forceinline__ void store_split_mirror(__half *base, int64_t pitch, int row0, int col, int rows, int cols_pad, int lane, const float (&v)[NC])
+{
+    // lane's element pair: columns row0 + (lane & ~1), + 1 of matrix row col + i + (lane & 1)
+    const int c = row0 + (lane & ~1);
+#pragma unroll
+    for (int i = 0; i < NC; i += 2)
+    {
+        const float give = (lane & 1) ? v[i] : v[i + 1];
+        const float got  = __shfl_xor_sync(0xffffffffu, give, 1);
+        const float x0 = (lane & 1) ? got : v[i], x1 = (lane & 1) ? v[i + 1] : got;
+        const int r = col + i + (lane & 1);
+        if (r < rows && c < cols_pad)
         {
-            muon_update_kernel<<<592, 256, 0, stream>>>(param + i * n, x, param_small ? param_small + i * n : nullptr, n, keep, rate);
-            ++g_launch_count;
+            uint32_t hi, lo;
+            s16::split2(x0, x1, hi, lo);
+            __half *p                            = base + r * pitch + (c >> 6) * 128 + (c & 63);
+            *reinterpret_cast<uint32_t *>(p)      = hi;
+            *reinterpret_cast<uint32_t *>(p + 64) = lo;
+        }
+    }
+}
+
+// A = X X^T or S = a I + b A + c A^2 (poly): symmetric, halves, both triangles
+template <bool POLY>
+struct EpiSym
+{
+    struct Params
+    {
+        __half *out;
+        const __half *a;  // POLY: A
+        int64_t pitch, stride;
+        int cols_pad;
+        float alpha;      // accumulator -> value * scale of the halves
+    };
+    template <int NC>
+    static __device__ __forceinline__ void store(const Params &p, const GemmArgs &, const TileAt &at, float (&v)[NC], float *)
+    {
+        const int64_t mat = at.batch * p.stride;
+        if (POLY)
+        {
+            const __half *row = p.a + mat + min(at.row, at.rows - 1) * p.pitch;
+            const float b     = at.row < at.rows ? kNsB * kSs / kSa : 0.f;  // (rows past the last mirror into padding: zeros)
+#pragma unroll
+            for (int i = 0; i < NC; i += 8)
+            {
+                const int c = min(at.col + i, p.cols_pad - 8);
+                const uint4 h = __ldg(reinterpret_cast<const uint4 *>(row + (c >> 6) * 128 + (c & 63)));
+                const uint4 l = __ldg(reinterpret_cast<const uint4 *>(row + (c >> 6) * 128 + (c & 63) + 64));
+                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const float2 fh = __half22float2(*reinterpret_cast<const __half2 *>(&hw[j]));
+                    const float2 fl = __half22float2(*reinterpret_cast<const __half2 *>(&lw[j]));
+                    v[i + 2 * j]     = fmaf(v[i + 2 * j], p.alpha, (fh.x + fl.x) * b);
+                    v[i + 2 * j + 1] = fmaf(v[i + 2 * j + 1], p.alpha, (fh.y + fl.y) * b);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (at.col + i == at.row && at.row < at.rows)
+                    v[i] += kNsA * kSs;
         }
         else
-            ODL_CUDA_TRY(cudaMemcpyAsync(out + i * n, x, n * 4, cudaMemcpyDeviceToDevice, stream));
-        ODL_CUDA_TRY(cudaGetLastError());
-        if ((rc = arena_end(stream)))
+        {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                v[i] *= p.alpha;
+        }
+        __half *out = p.out + mat;
+        if (at.row < at.rows)
+            store_split_row<NC>(out + at.row * p.pitch, at.col, p.cols_pad, v);
+        if (at.tm != at.tn)
+            store_split_mirror<NC>(out, p.pitch, at.row - at.lane, at.col, at.rows, p.cols_pad, at.lane, v);
+    }
+};
+
+// X of the next step, in halves
+struct EpiX
+{
+    struct Params
+    {
+        __half *out;
+        int64_t pitch, stride;
+        int cols_pad;
+        float alpha;
+    };
+    template <int NC>
+    static __device__ __forceinline__ void store(const Params &p, const GemmArgs &, const TileAt &at, float (&v)[NC], float *)
+    {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            v[i] *= p.alpha;
+        if (at.row < at.rows)
+            store_split_row<NC>(p.out + at.batch * p.stride + at.row * p.pitch, at.col, p.cols_pad, v);
+    }
+};
+
+// the last step's result: written out, or the parameters' update
+struct EpiOut
+{
+    struct Params
+    {
+        float *out;      // result, or parameters (param != 0)
+        float *small;    // low part of the parameters
+        int64_t ld, stride;
+        float alpha;     // accumulator -> X
+        float keep, rate;
+        int param, vec;
+    };
+    static __device__ __forceinline__ float one(const Params &p, float x, float was)
+    {
+        return p.param ? __fsub_rn(__fmul_rn(was, p.keep), __fmul_rn(p.rate, x * p.alpha)) : x * p.alpha;
+    }
+    template <int NC>
+    static __device__ __forceinline__ void store(const Params &p, const GemmArgs &g, const TileAt &at, float (&v)[NC], float *slab)
+    {
+        float *out   = p.out + at.batch * p.stride;
+        float *small = p.small ? p.small + at.batch * p.stride : nullptr;
+        if (p.vec)
+        {
+            if (at.row >= at.rows)
+                return;
+            float *row = out + at.row * p.ld + at.col;
+#pragma unroll
+            for (int i = 0; i < NC; i += 8)
+                if (at.col + i < g.N)  // (ld and with it N are multiples of 8)
+                {
+                    float was[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
+                    if (p.param)
+                        ld_global_v8(row + i, was);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        o[j] = one(p, v[i + j], was[j]);
+                    st_global_v8(row + i, o);
+                    if (small)
+                    {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            o[j] = tf32_small(o[j]);
+                        st_global_v8(small + at.row * p.ld + at.col + i, o);
+                    }
+                }
+            return;
+        }
+        const int row0 = at.row - at.lane;
+#pragma unroll
+        for (int b = 0; b < NC / 32; ++b)
+            s16::by_rows(v + 32 * b, slab, at.lane, [&](int r, float x) {
+                const int c = at.col + 32 * b + at.lane;
+                if (row0 + r < at.rows && c < g.N)
+                {
+                    const int64_t k = (row0 + r) * p.ld + c;
+                    const float o   = one(p, x, p.param ? out[k] : 0.f);
+                    out[k]          = o;
+                    if (small)
+                        small[k] = tf32_small(o);
+                }
+            });
+    }
+};
+
+// steps == 0: X_0 itself (the division alone)
+__global__ void __launch_bounds__(256) muon_direct_kernel(const __half *__restrict__ x, int64_t x_stride, int rows, int cols, int cols_pad,
+                                                          EpiOut::Params p)
+{
+    const int64_t n = static_cast<int64_t>(rows) * cols;
+    x += blockIdx.y * x_stride;
+    float *out   = p.out + blockIdx.y * p.stride;
+    float *small = p.small ? p.small + blockIdx.y * p.stride : nullptr;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    {
+        const int64_t r = i / cols;
+        const int c     = static_cast<int>(i - r * cols);
+        const __half *h = x + r * 2 * cols_pad + (c >> 6) * 128 + (c & 63);
+        const float o   = EpiOut::one(p, __half2float(h[0]) + __half2float(h[64]), p.param ? out[i] : 0.f);
+        out[i]          = o;
+        if (small)
+            small[i] = tf32_small(o);
+    }
+}
+
+template <class Epi>
+int gemm(const s16::Plan &plan, int terms, const Split16 &A, const Split16 &B, const GemmArgs &g, const typename Epi::Params &ep, cudaStream_t stream)
+{
+    return terms == 3 ? s16::launch_plan<3, false, Epi>(plan, A, B, g, ep, stream) : s16::launch_plan<1, false, Epi>(plan, A, B, g, ep, stream);
+}
+
+int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, EpiOut::Params out, int64_t batch, int64_t rows, int64_t cols,
+                  int steps, float eps, int precision, cudaStream_t stream)
+{
+    const int64_t n  = rows * cols;
+    const bool tall  = rows > cols;
+    const int64_t m  = tall ? cols : rows;
+    const int terms  = precision == ODL_PRECISION_3XTF32 ? 3 : 1;
+    const int xc = s16::pad64(cols), mc = s16::pad64(m);
+    // 256-byte multiples: rows are whole blocks of 64 columns
+    const int64_t x_stride = rows * 2 * xc, m_stride = m * 2 * mc;
+    int64_t blocks         = (n / 4 + 1023) / 1024;
+    blocks                 = blocks < 1 ? 1 : blocks > kNormBlocks ? kNormBlocks : blocks;
+    int rc = arena_begin(2 * a256(batch * x_stride * 2) + 2 * a256(batch * m_stride * 2) + a256(batch * blocks * 8), stream);
+    if (rc)
+        return rc;
+    __half *x[2]    = {static_cast<__half *>(arena_alloc(batch * x_stride * 2)), static_cast<__half *>(arena_alloc(batch * x_stride * 2))};
+    __half *A       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
+    __half *S       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
+    double *partial = static_cast<double *>(arena_alloc(batch * blocks * 8));
+    auto al16       = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    const bool vec  = !(n & 3) && al16(g) && al16(buf) && al16(p);
+    muon_momentum_kernel<<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, stream>>>(p, g, buf, n, a, vec, partial);
+    MUON_LAUNCHED();
+    int64_t sblocks = (rows * (xc / 64) + 31) / 32;
+    sblocks         = sblocks > 1184 ? 1184 : sblocks;
+    muon_split_kernel<<<dim3((unsigned)sblocks, (unsigned)batch), 256, 0, stream>>>(g, buf, (int)rows, (int)cols, xc, a.momentum, a.nesterov, partial,
+                                                                                   (int)blocks, eps, x[0], x_stride);
+    MUON_LAUNCHED();
+    out.ld = cols, out.stride = n;
+    out.vec = !(cols & 7) && !(reinterpret_cast<uintptr_t>(out.out) & 31) && !(reinterpret_cast<uintptr_t>(out.small) & 31);
+    if (steps == 0)
+    {
+        out.alpha = 1.f / kSx;
+        muon_direct_kernel<<<dim3((unsigned)sblocks, (unsigned)batch), 256, 0, stream>>>(x[0], x_stride, (int)rows, (int)cols, xc, out);
+        MUON_LAUNCHED();
+        return arena_end(stream);
+    }
+    GemmArgs gg{};
+    gg.batch = (int)batch, gg.splits = 1, gg.err = device_error_flag();
+    GemmArgs ga = gg, gs = gg, gx = gg;
+    ga.M = ga.N = (int)m, ga.K = (int)(tall ? rows : cols), ga.sym = 1, ga.a_mn = ga.b_mn = tall;
+    gs.M = gs.N = gs.K = (int)m, gs.sym = 1;
+    gx.M = (int)rows, gx.N = (int)cols, gx.K = (int)m, gx.b_mn = !tall;
+    const s16::Plan plan_a = s16::plan_tiles(m, m, ga.K, terms, (int)batch, false, true), plan_s = s16::plan_tiles(m, m, m, terms, (int)batch, false, true),
+                    plan_x = s16::plan_tiles(rows, cols, m, terms, (int)batch, false);
+    auto matrix = [&](const __half *d, int64_t r, int c_pad, int64_t stride) {
+        Split16 s;
+        s.data = d, s.pitch = 2 * c_pad, s.rows = (int)r, s.cols_pad = c_pad, s.batch = (int)batch, s.batch_stride = stride;
+        return s;
+    };
+    const Split16 MA = matrix(A, m, mc, m_stride), MS = matrix(S, m, mc, m_stride);
+    for (int k = 0; k < steps; ++k)
+    {
+        const Split16 MX = matrix(x[k & 1], rows, xc, x_stride);
+        const EpiSym<false>::Params ea{A, nullptr, 2 * mc, m_stride, mc, kSa / (kSx * kSx)};
+        const EpiSym<true>::Params es{S, A, 2 * mc, m_stride, mc, kNsC * kSs / (kSa * kSa)};
+        if ((rc = gemm<EpiSym<false>>(plan_a, terms, MX, MX, ga, ea, stream)) || (rc = gemm<EpiSym<true>>(plan_s, terms, MA, MA, gs, es, stream)))
+            return rc;
+        if (k + 1 < steps)
+        {
+            const EpiX::Params ex{x[(k + 1) & 1], 2 * xc, x_stride, xc, 1.f / kSs};
+            rc = gemm<EpiX>(plan_x, terms, tall ? MX : MS, tall ? MS : MX, gx, ex, stream);
+        }
+        else
+        {
+            out.alpha = 1.f / (kSs * kSx);
+            rc        = gemm<EpiOut>(plan_x, terms, tall ? MX : MS, tall ? MS : MX, gx, out, stream);
+        }
+        if (rc)
             return rc;
     }
-    return kOk;
+    return arena_end(stream);
 }
 
 int check_matrix(const char *what, int64_t batch, int64_t rows, int64_t cols, int steps, float eps, int precision)
@@ -201,8 +509,10 @@ extern "C" int odl_newton_schulz(const float *g, float *out, int64_t batch, int6
     if ((rc = check_ready()))
         return rc;
     const MomentumArgs a{0.f, 0.f, 1.f, 0};
-    return orthogonalise(nullptr, const_cast<float *>(g), nullptr, a, out, nullptr, nullptr, 1.f, 0.f, batch, rows, cols, steps, eps,
-                         precision, static_cast<cudaStream_t>(stream));
+    EpiOut::Params o{};
+    o.out = out;
+    return orthogonalise(nullptr, const_cast<float *>(g), nullptr, a, o, batch, rows, cols, steps, eps, precision,
+                         static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int odl_muon_step(float *param, float *grad, float *momentum_buf, float *param_small, int64_t batch, int64_t rows,
@@ -227,7 +537,10 @@ extern "C" int odl_muon_step(float *param, float *grad, float *momentum_buf, flo
     const double out = w_layout == ODL_W_OUT_IN ? rows : cols, in = w_layout == ODL_W_OUT_IN ? cols : rows;
     const double s   = out > in ? std::sqrt(out / in) : 1.0;
     const MomentumArgs a{momentum, hook_weight_decay, grad_scale, nesterov};
-    return orthogonalise(param, grad, momentum > 0.f ? momentum_buf : nullptr, a, nullptr, param, param_small,
-                         static_cast<float>(1.0 - static_cast<double>(lr) * weight_decay), static_cast<float>(lr * s), batch, rows,
-                         cols, steps, eps, precision, static_cast<cudaStream_t>(stream));
+    EpiOut::Params o{};
+    o.out = param, o.small = param_small, o.param = 1;
+    o.keep = static_cast<float>(1.0 - static_cast<double>(lr) * weight_decay);
+    o.rate = static_cast<float>(lr * s);
+    return orthogonalise(param, grad, momentum > 0.f ? momentum_buf : nullptr, a, o, batch, rows, cols, steps, eps, precision,
+                         static_cast<cudaStream_t>(stream));
 }

@@ -93,6 +93,40 @@ def test_values_and_gradients(ops, M, N, K, in_out):
     check(got, reference(x, w, t, b, in_out, 1.5, 0), ("loss", "lse", "dx", "dw", "db"))
 
 
+@pytest.fixture
+def chosen(ops):
+    """Sets the overrides of include/odl_b200_test.h and puts them back."""
+    from origindl_b200 import capi
+
+    def set_(tile=0, splits=0, piece=0):
+        capi.call("odl_debug_set_tile_n", tile)
+        capi.call("odl_debug_set_split_k", splits)
+        capi.call("odl_debug_set_loss_piece", piece)
+
+    yield set_
+    set_()
+
+
+@pytest.mark.parametrize("in_out", [False, True])
+@pytest.mark.parametrize("precision", [0, 1])
+@pytest.mark.parametrize("tile,splits,piece", [(64, 1, 0), (128, 1, 256), (256, 1, 0), (256, 3, 256), (128, 2, 0), (64, 5, 256)])
+def test_every_tile_and_split(ops, chosen, tile, splits, piece, precision, in_out):
+    x, w, t, b = make(600, 1100, 200, seed=tile + splits, in_out=in_out, bias=True, ignored=0.3)
+    chosen(tile, splits, piece)
+    got = ops.linear_cross_entropy(x, w, t, b=b, w_layout=ops.W_IN_OUT if in_out else ops.W_OUT_IN, precision=precision)
+    check(got, reference(x, w, t, b, in_out, 1.0, precision), ("loss", "lse", "dx", "dw", "db"))
+    got = ops.linear_cross_entropy(x, w, t, b=b, need_dx=False, need_dw=False, need_db=False, precision=precision,
+                                   w_layout=ops.W_IN_OUT if in_out else ops.W_OUT_IN)
+    check(got, reference(x, w, t, b, in_out, 1.0, precision), ("loss", "lse"))
+
+
+def test_pieces_with_few_rows_left(ops, chosen):
+    """Most rows are ignored: later pieces are empty, the first is not full."""
+    x, w, t, b = make(1300, 300, 100, seed=21, bias=True, ignored=0.97)
+    chosen(256, 1, 256)
+    check(ops.linear_cross_entropy(x, w, t, b=b), reference(x, w, t, b, False, 1.0, 0), ("loss", "lse", "dx", "dw", "db"))
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 777, 130), (7, 50021, 64), (40, 3000, 515), (300, 1111, 192), (2000, 300, 64)])
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
 def test_loss_alone(ops, M, N, K, itype):

@@ -91,6 +91,25 @@ def test_five_steps(ops, rows, cols):
     assert torch.linalg.matrix_norm(ops.newton_schulz(g).double() - want).item() <= far
 
 
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("rows,cols", [(300, 520), (777, 260), (130, 130), (64, 600)])
+def test_every_tile(ops, tile, rows, cols):
+    from origindl_b200 import capi
+
+    g = gradient(2, rows, cols, seed=tile)
+    capi.call("odl_debug_set_tile_n", tile)
+    try:
+        got = ops.newton_schulz(g)
+        plain = ops.newton_schulz(g, precision=ops.PRECISION_TF32)
+    finally:
+        capi.call("odl_debug_set_tile_n", 0)
+    for i in range(2):
+        want, far = bound(g[i], 5, 0)
+        assert torch.linalg.matrix_norm(got[i].double() - want).item() <= far
+        want, far = bound(g[i], 5, 1)
+        assert torch.linalg.matrix_norm(plain[i].double() - want).item() <= far
+
+
 @pytest.mark.parametrize("rows,cols", [(33, 70), (256, 512), (700, 300)])
 def test_plain_tf32(ops, rows, cols):
     g = gradient(rows, cols, seed=1)
