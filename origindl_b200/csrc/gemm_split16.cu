@@ -62,24 +62,29 @@ int resident_ctas(const void *kernel, int cluster, int smem)
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_split, bool sym)
 {
-    (void)terms;
+    // Times in units of a K-block of the pair's tile (1536 cycles with three products): a 128 x 128 tile's products take 0.5 of
+    // that on its SM, a 128 x 64 tile's 0.375 (shared-memory reads: 192 bytes a cycle for full rate, 128 there).  What the
+    // L2 -> SM fabric delivers, 10 MB a unit over all SMs, bounds the small tiles once many SMs run them: on 4096^3 the
+    // 128 x 128 tile kept the tensor pipe 57 % busy at 11 TB/s and took 386 us, the pair's tile 87 % and 309 us.
     struct Kind
     {
         int cg, bn;
-        double per_kb, fixed;  // of a tile: a K-block, and filling the ring + storing
+        double per_kb, bytes, fixed;  // of a tile: a K-block's products and bytes, filling the ring + storing
     };
-    const Kind kinds[3] = {{2, 256, 1.0, 4.0}, {1, 128, 0.52, 3.0}, {1, 64, 0.36, 2.5}};
+    const double parts  = terms == 3 ? 1.0 : 1.0 / 3;  // products; bytes are a half
+    const double bytes_ = terms == 3 ? 1.0 : 0.5;
+    const Kind kinds[3] = {{2, 256, 1.0, 131072, 4.0}, {1, 128, 0.5, 65536, 3.0}, {1, 64, 0.375, 49152, 2.5}};
     const int64_t n_kb  = (K + kBK - 1) / kBK;
-    const double sms    = sm_count();
     Plan best;
     double best_t = 1e300;
     for (const Kind &k : kinds)
     {
-        const int bm     = 128 * k.cg;
+        const int bm = 128 * k.cg;
         if (sym && bm != k.bn)
             continue;  // (a symmetric output needs square tiles)
         if (g_bn_override && (sym && g_bn_override == 64 ? 128 : g_bn_override) != k.bn)
             continue;
+        const int64_t slots = sm_count() / k.cg;
         const int64_t tn = (N + k.bn - 1) / k.bn, tm = (M + bm - 1) / bm;
         const int64_t tiles = (sym ? tn * (tn + 1) / 2 : tm * tn) * batch;
         for (int s = 1; s <= (may_split ? 16 : 1); ++s)
@@ -87,10 +92,15 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_
             const int64_t kb = (n_kb + s - 1) / s;
             if (may_split && g_split_k > 0 ? s != g_split_k : s > 1 && kb < 8)
                 continue;
-            const double slots = sms / k.cg;
-            const double waves = static_cast<double>((tiles * s + static_cast<int64_t>(slots) - 1) / static_cast<int64_t>(slots));
+            const int64_t units = tiles * s, waves = (units + slots - 1) / slots, full = units / slots;
+            const double busy = static_cast<double>(units < slots ? units : slots), rest = static_cast<double>(units - full * slots);
+            auto kb_time = [&](double active) {
+                const double fabric = active * k.bytes * bytes_ / 10e6;
+                return k.per_kb * parts > fabric ? k.per_kb * parts : fabric;
+            };
             // slices are written and read once more: M N s floats there and back
-            const double t = waves * (k.per_kb * kb + k.fixed) + (s > 1 ? 4.0 + static_cast<double>(M) * N * batch * s * 8 / 7e6 : 0.0);
+            const double t = (full * kb_time(busy) + (rest > 0 ? kb_time(rest) : 0.0)) * kb + waves * k.fixed +
+                             (s > 1 ? 4.0 + static_cast<double>(M) * N * batch * s * 8 / 5e6 : 0.0);
             if (t < best_t)
                 best_t = t, best.cg = k.cg, best.bn = k.bn, best.splits = s;
         }

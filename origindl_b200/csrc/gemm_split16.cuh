@@ -102,6 +102,14 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo               = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// 2^x to 2^-22 of itself, 0 below the normal range
+__device__ __forceinline__ float fast_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <int CG, int BN, int TERMS>
 struct Cfg
 {
@@ -516,9 +524,7 @@ int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::P
     return kOk;
 }
 
-// Which tile and how many slices of the reduction.  Times in units of one K-block of a 256 x 256 tile on a CTA pair
-// (3 x 256 x 256 x 64 products on two SMs): a 128 x 128 tile does half of that per SM, a 128 x 64 tile a quarter of it, but is
-// held back by shared-memory reads (192 bytes a cycle for full rate against 128).
+// Which tile and how many slices of the reduction, by the estimate in plan_tiles.
 struct Plan
 {
     int cg = 2, bn = 256, splits = 1;

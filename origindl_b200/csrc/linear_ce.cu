@@ -194,20 +194,27 @@ struct EpiLogits
                     st_global_v8(row + i, o);
                 }
         }
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
+        if (at.col + NC > g.N)
         {
-            v[i] = at.col + i < g.N ? v[i] : -INFINITY;
-            m    = fmaxf(m, v[i]);
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                v[i] = at.col + i < g.N ? v[i] : -INFINITY;
         }
+        float m = v[0], m1 = v[1];
+#pragma unroll
+        for (int i = 2; i < NC; i += 2)
+        {
+            m  = fmaxf(m, v[i]);
+            m1 = fmaxf(m1, v[i + 1]);
+        }
+        m = fmaxf(m, m1);
         const float base = m == -INFINITY ? 0.f : m;  // a strip without a class left: sum 0, not NaN
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int i = 0; i < NC; i += 2)
         {
-            s0 += exp2f((v[i] - base) * kLog2e);
-            s1 += exp2f((v[i + 1] - base) * kLog2e);
+            s0 += s16::fast_exp2((v[i] - base) * kLog2e);
+            s1 += s16::fast_exp2((v[i + 1] - base) * kLog2e);
         }
         if (live)
             p.part[static_cast<int64_t>(at.strip) * p.part_ld + at.row] = make_float2(m, s0 + s1);
@@ -353,8 +360,8 @@ __global__ void __launch_bounds__(256) lce_softmax_kernel(float *z, int64_t ld, 
             const bool on  = r + i < live - r0;
             const float l  = s_lse[r + i];
             const int t    = s_cls[r + i] - c;
-            float a        = on && c < N ? exp2f((v[i].x - l) * kLog2e) : 0.f;
-            float b        = on && c + 1 < N ? exp2f((v[i].y - l) * kLog2e) : 0.f;
+            float a        = on && c < N ? s16::fast_exp2((v[i].x - l) * kLog2e) : 0.f;
+            float b        = on && c + 1 < N ? s16::fast_exp2((v[i].y - l) * kLog2e) : 0.f;
             a -= t == 0 ? 1.f : 0.f;
             b -= t == 1 ? 1.f : 0.f;
             sum.x += a;
