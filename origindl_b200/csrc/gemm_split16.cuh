@@ -144,9 +144,8 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
     uint8_t *tiles      = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *slabs        = reinterpret_cast<float *>(tiles + C::stages * C::stage);
     uint64_t *full_bar  = reinterpret_cast<uint64_t *>(tiles + C::stages * C::stage + kEpi * kSlab);
-    uint64_t *empty_bar = full_bar + C::stages;
-    uint64_t *acc_full  = empty_bar + C::stages;
-    uint64_t *acc_empty = acc_full + 2;
+    uint64_t *done_bar  = full_bar + C::stages;  // a stage's MMAs are complete: its buffers are free, its accumulator is full
+    uint64_t *acc_empty = done_bar + C::stages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     volatile int *abort_f = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *early_out        = const_cast<int *>(abort_f) + 1;
@@ -162,13 +161,10 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
         for (int s = 0; s < C::stages; ++s)
         {
             ptx::mbar_init(&full_bar[s], 1);
-            ptx::mbar_init(&empty_bar[s], 1);
+            ptx::mbar_init(&done_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b)
-        {
-            ptx::mbar_init(&acc_full[b], 1);
             ptx::mbar_init(&acc_empty[b], CG * kEpi);
-        }
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm.a);
         ptx::prefetch_tmap(&tm.b);
@@ -261,7 +257,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                 for (int kb = kb0; kb < kb1; ++kb, ++gk)
                 {
                     const int s = gk % C::stages;
-                    if (!ptx::mbar_wait(&empty_bar[s], ((gk / C::stages) & 1) ^ 1, abort_f))
+                    if (!ptx::mbar_wait(&done_bar[s], ((gk / C::stages) & 1) ^ 1, abort_f))
                     {
                         ok = false;
                         break;
@@ -354,15 +350,9 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                     for (int k = 0; k < kBK / 16; ++k)
                         mma(sa + k * a_step, sb + k * b_step, TERMS == 3 || k != 0);
                     if (CG == 2)
-                    {
-                        ptx::mma_commit_pair_both(&empty_bar[s]);
-                        ptx::mma_commit_pair_both(&acc_full[buf]);
-                    }
+                        ptx::mma_commit_pair_both(&done_bar[s]);
                     else
-                    {
-                        ptx::mma_commit(&empty_bar[s]);
-                        ptx::mma_commit(&acc_full[buf]);
-                    }
+                        ptx::mma_commit(&done_bar[s]);
                 }
             }
         }
@@ -399,7 +389,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
             };
             for (int kb = kb0; kb < kb1; ++kb, ++gc)
             {
-                const int buf = gc & 1;
+                const int buf = gc & 1, s = gc % C::stages;
                 float f0 = 1.f, f1 = 1.f;
                 if (SCALED)
                 {
@@ -407,7 +397,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                     f0            = a * (g.sb ? scale_b(kb, 0) : 1.f);
                     f1            = C::strip > 64 ? a * (g.sb ? scale_b(kb, 1) : 1.f) : f0;
                 }
-                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[buf], (gc >> 1) & 1, abort_f));
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&done_bar[s], (gc / C::stages) & 1, abort_f));
                 if (!ok)
                     break;
                 ptx::tc_fence_after_sync();
