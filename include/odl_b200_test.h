@@ -45,7 +45,8 @@ int odl_debug_set_stream_k(int mode);
  * 8 = four input channels per thread in the compile-time input-gradient kernels where they would take eight. */
 int odl_debug_set_conv_mode(int mode);
 
-/* odl_linear_cross_entropy: rows whose logits are held at a time, rounded up to a multiple of 256; 0 = automatic.  (Its GEMMs
+/* odl_linear_cross_entropy: rows whose logits are held at a time, rounded up to a multiple of 256; 0 = automatic
+ * (also: the form for few rows where it applies).  (Its GEMMs
  * and those of odl_newton_schulz follow odl_debug_set_tile_n -- 256 is their CTA-pair tile -- and a positive
  * odl_debug_set_split_k.) */
 int odl_debug_set_loss_piece(int rows);

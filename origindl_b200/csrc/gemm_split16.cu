@@ -115,9 +115,11 @@ namespace
 template <bool TRANSPOSED>
 __global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restrict__ src, int64_t ld, int rows, int cols, const int *__restrict__ gather,
                                                             const int *__restrict__ count, __half *__restrict__ out, int64_t pitch,
-                                                            float *__restrict__ scale, bool vec)
+                                                            float *__restrict__ scale, int blocks_c, bool vec)
 {
-    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 128;
+    // neighbouring blocks take neighbouring columns: rows are read in long stretches (DRAM pages), not 256 bytes at a time
+    const int block_c = blockIdx.x % blocks_c, block_r = blockIdx.x / blocks_c;
+    const int c0 = block_c * 64, r0 = block_r * 128;
     const int live = count ? min(rows, *count) : rows;
     if (r0 >= live)
         return;  // (gathered matrices: nobody reads rows past the last 128 that hold any)
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restr
     const float s   = __int_as_float((e - 14 + 127) << 23);
     const float inv = __int_as_float((127 - (e - 14)) << 23);
     if (threadIdx.x == 0)
-        scale[static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y] = s;
+        scale[blockIdx.x] = s;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
     {
@@ -210,18 +212,20 @@ __global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restr
 int split16_encode(const float *src, int64_t ld, int transposed, int rows, int cols, const int *gather, const int *count, const Split16 &out,
                    float *scale, cudaStream_t stream)
 {
-    const dim3 grid((rows + 127) / 128, out.cols_pad / 64);
-    if (grid.y > 65535)
+    const int blocks_c   = out.cols_pad / 64;
+    const int64_t blocks = static_cast<int64_t>((rows + 127) / 128) * blocks_c;
+    if (blocks > 0x7fffffff)
     {
-        set_last_error("split: %d columns exceed 65535 blocks of 64", cols);
+        set_last_error("split: %d x %d is too large", rows, cols);
         return kTooLarge;
     }
+    const unsigned grid = static_cast<unsigned>(blocks);
     const bool vec = !(cols & 1) && !(ld & 1) && !(reinterpret_cast<uintptr_t>(src) & 7);
     __half *dst    = const_cast<__half *>(out.data);
     if (transposed)
-        split16_tiles_kernel<true><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, vec);
+        split16_tiles_kernel<true><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, blocks_c, vec);
     else
-        split16_tiles_kernel<false><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, vec);
+        split16_tiles_kernel<false><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, blocks_c, vec);
     ++g_launch_count;
     ODL_CUDA_TRY(cudaGetLastError());
     return kOk;

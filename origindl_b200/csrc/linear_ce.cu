@@ -22,6 +22,7 @@
 #include "gemm_split16.cuh"
 #include "host_util.h"
 #include "internal.h"
+#include "linear_ce.h"
 #include "split16_encode.h"
 
 namespace odl
@@ -477,6 +478,8 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     }
     const int terms    = precision == ODL_PRECISION_3XTF32 ? 3 : 1;
     const bool grads   = dx || dw || db;
+    if (!grads && !g_lce_piece && linear_ce_few_eligible(M, N, K, w, w_layout))
+        return linear_ce_few(x, w, b, labels, is64, ignore_index, M, N, K, w_layout, loss, lse_out, precision, stream);
     const bool out_in  = w_layout == ODL_W_OUT_IN;
     const int kp = s16::pad64(K), np = s16::pad64(N);
     const int64_t m_pad = (M + 127) / 128 * 128;

@@ -127,6 +127,44 @@ def test_pieces_with_few_rows_left(ops, chosen):
     check(ops.linear_cross_entropy(x, w, t, b=b), reference(x, w, t, b, False, 1.0, 0), ("loss", "lse", "dx", "dw", "db"))
 
 
+@pytest.mark.parametrize("in_out", [False, True])
+@pytest.mark.parametrize("precision", [0, 1])
+@pytest.mark.parametrize("M,N,K", [(1, 4, 4), (1, 1, 1), (1, 7, 3), (2, 1001, 77), (3, 130, 999), (4, 50021, 65), (5, 999, 4001), (8, 5001, 130),
+                                   (8, 40000, 64), (8, 300, 7000), (1, 20, 8), (1, 5000, 2048), (2, 128, 32), (9, 2500, 36), (15, 132, 100), (16, 4096, 64), (17, 33000, 96),
+                                   (32, 1000, 260), (33, 7000, 128), (48, 19000, 64), (64, 300, 1000), (64, 40000, 68)])
+def test_few_rows(ops, M, N, K, precision, in_out):
+    """Up to 64 rows without gradients: read straight from the weights (aligned ones above 8 rows)."""
+    x, w, t, b = make(M, N, K, seed=N, in_out=in_out, bias=True, ignored=0.3 if M > 4 else 0.0, sharp=3.0)
+    got = ops.linear_cross_entropy(x, w, t, b=b, need_dx=False, need_dw=False, need_db=False, precision=precision,
+                                   w_layout=ops.W_IN_OUT if in_out else ops.W_OUT_IN)
+    check(got, reference(x, w, t, b, in_out, 1.0, precision), ("loss", "lse"))
+
+
+def test_few_rows_garbage_masks_and_bad_labels(ops):
+    from origindl_b200 import capi
+
+    x, w, t, b = make(20, 3000, 64, seed=30, bias=True)
+    t[::3] = -100
+    x[::3] = float("nan")
+    b[:2000] = float("-inf")
+    t[t != -100] = 2500
+    kw = dict(need_dx=False, need_dw=False, need_db=False)
+    got = ops.linear_cross_entropy(x, w, t, b=b, **kw)
+    want = reference(x, w[2000:].contiguous(), torch.where(t == -100, t, t - 2000), b[2000:].contiguous(), False, 1.0, 0)
+    check(got, want, ("loss", "lse"))
+    bad = t.clone()
+    bad[1] = 3000
+    t[1] = -100
+    got = ops.linear_cross_entropy(x, w, bad, b=b, **kw)
+    with pytest.raises(capi.OdlError, match="linear_cross_entropy"):
+        capi.device_status()
+    for u, v in zip(got[:2], ops.linear_cross_entropy(x, w, t, b=b, **kw)[:2]):
+        assert torch.equal(u, v)
+    t.fill_(-100)
+    loss, lse = ops.linear_cross_entropy(x, w, t, b=b, **kw)[:2]
+    assert loss == 0 and (lse == 0).all()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 777, 130), (7, 50021, 64), (40, 3000, 515), (300, 1111, 192), (2000, 300, 64)])
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
 def test_loss_alone(ops, M, N, K, itype):
