@@ -111,73 +111,86 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_
 namespace
 {
 // One 128 x 64 tile per block: read once, its largest finite value gives the tile's power of two, written as halves.
-// Bound by memory: 4 bytes in and 4 out per value.  TRANSPOSED: element (r, c) is src[c * ld + r].
-template <bool TRANSPOSED>
-__global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restrict__ src, int64_t ld, int rows, int cols, const int *__restrict__ gather,
-                                                            const int *__restrict__ count, __half *__restrict__ out, int64_t pitch,
-                                                            float *__restrict__ scale, int blocks_c, bool vec)
+// Bound by memory: 4 bytes in and 4 out per value.  A launch holds two matrices (x and W of a loss) and a range of blocks that
+// put zeros into rows of `zero` and words of `zero_lse` (rows without a label: pos_of < 0).
+__device__ __forceinline__ void split16_tile(const EncodeJob &j, int block, float (&box)[8], float (&tile)[64][129])
 {
-    // neighbouring blocks take neighbouring columns: rows are read in long stretches (DRAM pages), not 256 bytes at a time
-    const int block_c = blockIdx.x % blocks_c, block_r = blockIdx.x / blocks_c;
+    // neighbouring blocks take neighbouring columns: rows are read in long stretches
+    const int block_c = block % j.blocks_c, block_r = block / j.blocks_c;
     const int c0 = block_c * 64, r0 = block_r * 128;
-    const int live = count ? min(rows, *count) : rows;
+    const int live = j.count ? min(j.rows, *j.count) : j.rows;
     if (r0 >= live)
         return;  // (gathered matrices: nobody reads rows past the last 128 that hold any)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float2 v[16];
-    if (TRANSPOSED)
+    // thread: rows (lane / 16) + 2 warp + 16 i, columns 4 (lane % 16) .. + 3 of the tile
+    const int cc = 4 * (lane & 15), rr = 2 * warp + (lane >> 4);
+    float4 v[8];
+    if (j.transposed)
     {
-        __shared__ float tile[64][129];
+        const bool vec = !(j.ld & 3) && !(reinterpret_cast<uintptr_t>(j.src) & 15) && r0 + 128 <= live;
         for (int i = warp; i < 64; i += 8)
         {
-            const float *line = src + (c0 + i) * ld + r0;
-            for (int j = 0; j < 4; ++j)
+            const float *line = j.src + (c0 + i) * j.ld + r0;
+            if (vec && c0 + i < j.cols)
             {
-                const int r           = lane + 32 * j;
-                tile[i][r] = (c0 + i < cols && r0 + r < live) ? __ldg(line + r) : 0.f;
+                const float4 q = __ldg(reinterpret_cast<const float4 *>(line) + lane);
+                tile[i][4 * lane] = q.x, tile[i][4 * lane + 1] = q.y, tile[i][4 * lane + 2] = q.z, tile[i][4 * lane + 3] = q.w;
             }
+            else
+                for (int k = 0; k < 4; ++k)
+                {
+                    const int r = lane + 32 * k;
+                    tile[i][r]  = (c0 + i < j.cols && r0 + r < live) ? __ldg(line + r) : 0.f;
+                }
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            v[i] = make_float2(tile[2 * lane][warp + 8 * i], tile[2 * lane + 1][warp + 8 * i]);
+        for (int i = 0; i < 8; ++i)
+        {
+            const int r = rr + 16 * i;
+            v[i]        = make_float4(tile[cc][r], tile[cc + 1][r], tile[cc + 2][r], tile[cc + 3][r]);
+        }
     }
     else
     {
-        const int c = c0 + 2 * lane;
+        const int c    = c0 + cc;
+        const bool vec = !(j.ld & 3) && !(j.cols & 3) && !(reinterpret_cast<uintptr_t>(j.src) & 15);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 8; ++i)
         {
-            const int r = r0 + warp + 8 * i;
-            v[i]        = make_float2(0.f, 0.f);
+            const int r = r0 + rr + 16 * i;
+            v[i]        = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < live)
             {
-                const float *line = src + static_cast<int64_t>(gather ? gather[r] : r) * ld;
+                const float *line = j.src + static_cast<int64_t>(j.gather ? j.gather[r] : r) * j.ld + c;
                 if (vec)
                 {
-                    if (c < cols)
-                        v[i] = __ldg(reinterpret_cast<const float2 *>(line + c));
+                    if (c < j.cols)
+                        v[i] = __ldg(reinterpret_cast<const float4 *>(line));
                 }
                 else
                 {
-                    if (c < cols)
-                        v[i].x = __ldg(line + c);
-                    if (c + 1 < cols)
-                        v[i].y = __ldg(line + c + 1);
+                    if (c < j.cols)
+                        v[i].x = __ldg(line);
+                    if (c + 1 < j.cols)
+                        v[i].y = __ldg(line + 1);
+                    if (c + 2 < j.cols)
+                        v[i].z = __ldg(line + 2);
+                    if (c + 3 < j.cols)
+                        v[i].w = __ldg(line + 3);
                 }
             }
         }
     }
     float top = 0.f;
+    // infinities and NaN stay what they are and choose no scale
+    auto see = [&](float x) {
+        x   = fabsf(x);
+        top = fmaxf(top, x < INFINITY ? x : 0.f);
+    };
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-    {
-        // infinities and NaN stay what they are and choose no scale
-        const float a = fabsf(v[i].x), b = fabsf(v[i].y);
-        top = fmaxf(top, a < INFINITY ? a : 0.f);
-        top = fmaxf(top, b < INFINITY ? b : 0.f);
-    }
-    __shared__ float box[8];
+    for (int i = 0; i < 8; ++i)
+        see(v[i].x), see(v[i].y), see(v[i].z), see(v[i].w);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -192,43 +205,69 @@ __global__ void __launch_bounds__(256) split16_tiles_kernel(const float *__restr
     const float s   = __int_as_float((e - 14 + 127) << 23);
     const float inv = __int_as_float((127 - (e - 14)) << 23);
     if (threadIdx.x == 0)
-        scale[blockIdx.x] = s;
+        j.scale[block] = s;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
     {
-        const int r = r0 + warp + 8 * i;
-        if (r < (gather ? r0 + 128 : rows))
+        const int r = r0 + rr + 16 * i;
+        if (r < (j.gather ? r0 + 128 : j.rows))
         {
-            uint32_t hi, lo;
-            split2(v[i].x * inv, v[i].y * inv, hi, lo);
-            uint32_t *line = reinterpret_cast<uint32_t *>(out + r * pitch + 2 * c0);
-            line[lane]      = hi;
-            line[32 + lane] = lo;
+            uint2 hi, lo;
+            split2(v[i].x * inv, v[i].y * inv, hi.x, lo.x);
+            split2(v[i].z * inv, v[i].w * inv, hi.y, lo.y);
+            __half *line = j.out + r * j.pitch + 2 * c0 + cc;
+            *reinterpret_cast<uint2 *>(line)      = hi;
+            *reinterpret_cast<uint2 *>(line + 64) = lo;
         }
+    }
+}
+
+__global__ void __launch_bounds__(256) split16_tiles_kernel(const __grid_constant__ EncodeJob a, const __grid_constant__ EncodeJob b, const ZeroRows z)
+{
+    __shared__ float box[8];
+    __shared__ float tile[64][129];
+    let_next_in();
+    after_previous();
+    int block = blockIdx.x;
+    if (block < a.blocks)
+        return split16_tile(a, block, box, tile);
+    block -= a.blocks;
+    if (block < b.blocks)
+        return split16_tile(b, block, box, tile);
+    block -= b.blocks;
+    const int lane = threadIdx.x & 31;
+    for (int row = block * 8 + (threadIdx.x >> 5); row < z.rows; row += z.blocks * 8)
+    {
+        if (z.pos_of[row] >= 0)
+            continue;
+        if (z.words && lane == 0)
+            z.words[row] = 0.f;
+        if (z.matrix)
+            for (int c = lane; c < z.cols; c += 32)
+                z.matrix[static_cast<int64_t>(row) * z.cols + c] = 0.f;
     }
 }
 }  // namespace
 
-int split16_encode(const float *src, int64_t ld, int transposed, int rows, int cols, const int *gather, const int *count, const Split16 &out,
-                   float *scale, cudaStream_t stream)
+EncodeJob encode_job(const float *src, int64_t ld, int transposed, int rows, int cols, const int *gather, const int *count, const Split16 &out, float *scale)
 {
-    const int blocks_c   = out.cols_pad / 64;
-    const int64_t blocks = static_cast<int64_t>((rows + 127) / 128) * blocks_c;
+    EncodeJob j;
+    j.src = src, j.ld = ld, j.transposed = transposed, j.rows = rows, j.cols = cols, j.gather = gather, j.count = count;
+    j.out = const_cast<__half *>(out.data), j.pitch = out.pitch, j.scale = scale;
+    j.blocks_c = out.cols_pad / 64;
+    j.blocks   = static_cast<int64_t>((rows + 127) / 128) * j.blocks_c;
+    return j;
+}
+
+int split16_encode(const EncodeJob &a, const EncodeJob &b, const ZeroRows &z, cudaStream_t stream)
+{
+    const int64_t blocks = a.blocks + b.blocks + z.blocks;
     if (blocks > 0x7fffffff)
     {
-        set_last_error("split: %d x %d is too large", rows, cols);
+        set_last_error("split: %lld tiles are too many", (long long)blocks);
         return kTooLarge;
     }
-    const unsigned grid = static_cast<unsigned>(blocks);
-    const bool vec = !(cols & 1) && !(ld & 1) && !(reinterpret_cast<uintptr_t>(src) & 7);
-    __half *dst    = const_cast<__half *>(out.data);
-    if (transposed)
-        split16_tiles_kernel<true><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, blocks_c, vec);
-    else
-        split16_tiles_kernel<false><<<grid, 256, 0, stream>>>(src, ld, rows, cols, gather, count, dst, out.pitch, scale, blocks_c, vec);
-    ++g_launch_count;
-    ODL_CUDA_TRY(cudaGetLastError());
-    return kOk;
+    return launch_after(split16_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, b, z);
 }
 
 }  // namespace s16

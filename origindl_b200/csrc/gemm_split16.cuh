@@ -110,6 +110,18 @@ __device__ __forceinline__ float fast_exp2(float x)
     return y;
 }
 
+// Programmatic launches: a kernel of these operators may be resident before the one in front of it has finished; it sets itself
+// up (barriers, TMEM, tensor maps) and then waits here for that one's results.  Every kernel launched with launch_after() calls
+// both, so that completion carries over from kernel to kernel.
+__device__ __forceinline__ void after_previous()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_in()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 template <int CG, int BN, int TERMS>
 struct Cfg
 {
@@ -154,6 +166,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
     const uint32_t rank = CG == 2 ? ptx::cluster_ctarank() : 0u;
     const bool leader   = rank == 0;
 
+    let_next_in();
     if (threadIdx.x == 0)
     {
         *early_out = (leader && *reinterpret_cast<volatile int *>(g.err) == 1) ? 1 : 0;  // an earlier wait gave up
@@ -190,6 +203,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
     const uint32_t tmem_base = *tmem_slot;
     const bool skip = CG == 2 ? ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(early_out), 0)) != 0 : *early_out != 0;
 
+    after_previous();
     int M = g.M, K = g.K;
     if (g.count)
     {
@@ -466,6 +480,31 @@ int make_tmap_split16(CUtensorMap *out, const Split16 &m, int box_rows);
 int sm_count();
 int resident_ctas(const void *kernel, int cluster, int smem);
 
+// kernel<<<grid, block, smem, stream>>>(args...) as a programmatic launch (see after_previous)
+template <class... P, class... A>
+int launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim          = grid;
+    cfg.blockDim         = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream           = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs       = attr;
+    cfg.numAttrs    = 1;
+    cudaError_t e   = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    ++g_launch_count;
+    if (e != cudaSuccess)
+    {
+        set_last_error("kernel launch failed: %s", cudaGetErrorString(e));
+        return kCudaError;
+    }
+    return kOk;
+}
+
 template <int CG, int BN, int TERMS, bool SCALED, class Epi>
 int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::Params &ep, cudaStream_t stream)
 {
@@ -497,13 +536,15 @@ int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::P
     cfg.blockDim         = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::smem;
     cfg.stream           = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id               = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs                = attr;
-    cfg.numAttrs             = 1;
+    cfg.numAttrs             = 2;
     cudaError_t e            = cudaLaunchKernelEx(&cfg, kernel, tm, g, ep);
     ++g_launch_count;
     if (e != cudaSuccess)

@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(1024) lce_labels_kernel(const void *__restrict
                                                           Counters *out)
 {
     __shared__ int warp_sum[32], base, any_bad;
+    s16::let_next_in();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0)
         base = 0, any_bad = 0;
@@ -130,22 +131,6 @@ __global__ void __launch_bounds__(1024) lce_labels_kernel(const void *__restrict
         out->count     = base;
         out->inv_count = base > 0 ? 1.0f / static_cast<float>(base) : 0.f;
         out->bad       = any_bad;
-    }
-}
-
-// rows without a label: lse = 0, dx = 0 (one warp per row)
-__global__ void __launch_bounds__(256) lce_ignored_kernel(const int *__restrict__ pos_of, int M, int K, float *__restrict__ lse, float *__restrict__ dx)
-{
-    const int lane = threadIdx.x & 31;
-    for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < M; row += gridDim.x * 8)
-    {
-        if (pos_of[row] >= 0)
-            continue;
-        if (lse && lane == 0)
-            lse[row] = 0.f;
-        if (dx)
-            for (int c = lane; c < K; c += 32)
-                dx[static_cast<int64_t>(row) * K + c] = 0.f;
     }
 }
 
@@ -283,61 +268,105 @@ struct EpiGrad
     }
 };
 
-// lse of each row of a piece from its strips' maxima and sums (32 rows x 8 groups of strips per block), and the row's loss
-__global__ void __launch_bounds__(256) lce_lse_kernel(const float2 *__restrict__ part, int part_ld, int strips, int rows, int base, const Counters *cnt,
-                                                      const int *__restrict__ idx, const float *__restrict__ picked, float *__restrict__ lse,
-                                                      float *__restrict__ row_loss, float *__restrict__ lse_out)
+__device__ __forceinline__ void join(float &m, float &s, float om, float os)
 {
-    const int live = min(rows, cnt->count - base);
-    const int row = blockIdx.x * 32 + (threadIdx.x & 31), part_of = threadIdx.x >> 5;
+    const float t = fmaxf(m, om), b = t == -INFINITY ? 0.f : t;
+    s = s * s16::fast_exp2((m - b) * kLog2e) + os * s16::fast_exp2((om - b) * kLog2e);
+    m = t;
+}
+
+struct LseArgs
+{
+    const float2 *part;  // [strip][part_ld]
+    int part_ld, strips;
+    int rows, base;      // of the piece; its first row among those with a label
+    const Counters *cnt;
+    const int *idx;      // of the piece's rows
+    const float *picked;
+    float *lse, *row_loss, *lse_out;
+};
+
+// lse of 32 rows of a piece from their strips' maxima and sums, by GROUPS warps (lane = row), and the rows' losses
+template <int GROUPS>
+__device__ __forceinline__ void lse_of_rows(const LseArgs &p, int row0, int live, float2 (&box)[GROUPS][32], float *s_lse)
+{
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, row = row0 + lane;
     float m = -INFINITY, s = 0.f;
     if (row < live)
-        for (int k = part_of; k < strips; k += 8)
-        {
-            const float2 p = part[static_cast<int64_t>(k) * part_ld + row];
-            const float t  = fmaxf(m, p.x);
-            const float b  = t == -INFINITY ? 0.f : t;
-            s              = s * exp2f((m - b) * kLog2e) + p.y * exp2f((p.x - b) * kLog2e);
-            m              = t;
-        }
-    __shared__ float2 box[8][32];
-    box[part_of][threadIdx.x & 31] = make_float2(m, s);
-    __syncthreads();
-    if (part_of == 0 && row < live)
     {
-        for (int k = 1; k < 8; ++k)
+        const float2 *src = p.part + row;
+        int k             = group;
+        for (; k + 3 * GROUPS < p.strips; k += 4 * GROUPS)
         {
-            const float2 p = box[k][threadIdx.x];
-            const float t  = fmaxf(m, p.x);
-            const float b  = t == -INFINITY ? 0.f : t;
-            s              = s * exp2f((m - b) * kLog2e) + p.y * exp2f((p.x - b) * kLog2e);
-            m              = t;
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = src[static_cast<int64_t>(k + i * GROUPS) * p.part_ld];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                join(m, s, v[i].x, v[i].y);
         }
-        const float l        = m + logf(s);
-        lse[row]             = l;
-        row_loss[base + row] = l - picked[row];
-        if (lse_out)
-            lse_out[idx[row]] = l;
+        for (; k < p.strips; k += GROUPS)
+        {
+            const float2 v = src[static_cast<int64_t>(k) * p.part_ld];
+            join(m, s, v.x, v.y);
+        }
+    }
+    box[group][lane] = make_float2(m, s);
+    __syncthreads();
+    if (group == 0)
+    {
+        if (row < live)
+        {
+            for (int k = 1; k < GROUPS; ++k)
+                join(m, s, box[k][lane].x, box[k][lane].y);
+            const float l = m + logf(s);
+            if (s_lse)
+                s_lse[lane] = l;
+            else
+                p.lse[row] = l;
+            p.row_loss[p.base + row] = l - p.picked[row];
+            if (p.lse_out)
+                p.lse_out[p.idx[row]] = l;
+        }
+        else if (s_lse)
+            s_lse[lane] = 0.f;
     }
 }
 
-// Logits of a piece -> P * 2^15 in halves, in place.  A block: 512 columns (a warp per block of 64) x 128 rows; a warp reads the
-// 256 bytes of 64 logits and writes the same 256 bytes as [64 hi][64 lo].  Rows behind the last (up to a multiple of 128) and
-// padding columns become zeros.  colsum (optional): sums of P over the block's rows, [row block][ld].
-__global__ void __launch_bounds__(256) lce_softmax_kernel(float *z, int64_t ld, int N, int rows, int base, const Counters *cnt,
-                                                          const float *__restrict__ lse, const int *__restrict__ cls, float *__restrict__ colsum)
+__global__ void __launch_bounds__(512) lce_lse_kernel(const LseArgs p)
 {
-    __shared__ float s_lse[128];
-    __shared__ int s_cls[128];
-    const int r0 = blockIdx.x * 128, live = min(rows, cnt->count - base);
-    if (r0 >= live)
+    __shared__ float2 box[16][32];
+    s16::let_next_in();
+    s16::after_previous();
+    lse_of_rows<16>(p, blockIdx.x * 32, min(p.rows, p.cnt->count - p.base), box, nullptr);
+}
+
+// Logits of a piece -> P * 2^15 in halves, in place.  A block: 512 columns (a warp per block of 64) x ROWS rows; a warp reads the
+// 256 bytes of 64 logits and writes the same 256 bytes as [64 hi][64 lo].  Rows behind the last (up to a multiple of 128) and
+// padding columns become zeros.  colsum (optional): sums of P over the block's rows, [row block][ld].  ROWS = 32: pieces whose
+// 128-row blocks would leave SMs idle; there, and with one block over the columns, the block finds its rows' lse itself.
+template <int ROWS>
+__global__ void __launch_bounds__(256) lce_softmax_kernel(float *z, int64_t ld, int N, int rows, const LseArgs p, const int *__restrict__ cls, int own_lse,
+                                                          float *__restrict__ colsum)
+{
+    __shared__ float s_lse[ROWS];
+    __shared__ int s_cls[ROWS];
+    __shared__ float2 box[8][32];
+    s16::let_next_in();
+    s16::after_previous();
+    const int r0 = blockIdx.x * ROWS, live = min(p.rows, p.cnt->count - p.base);
+    if (r0 >= (live + 127) / 128 * 128)
         return;
-    if (threadIdx.x < 128)
+    if (threadIdx.x < ROWS)
     {
-        const int r        = r0 + threadIdx.x;
-        s_lse[threadIdx.x] = r < live ? lse[r] : 0.f;
+        const int r = r0 + threadIdx.x;
+        if (!own_lse)
+            s_lse[threadIdx.x] = r < live ? p.lse[r] : 0.f;
         s_cls[threadIdx.x] = r < live ? cls[r] : -1;
     }
+    if (ROWS == 32 && own_lse)
+        lse_of_rows<8>(p, r0, live, box, s_lse);
     __syncthreads();
     const int lane = threadIdx.x & 31;
     const int c0   = blockIdx.y * 512 + (threadIdx.x >> 5) * 64;
@@ -345,7 +374,7 @@ __global__ void __launch_bounds__(256) lce_softmax_kernel(float *z, int64_t ld, 
         return;
     const int c = c0 + 2 * lane;
     float2 sum  = make_float2(0.f, 0.f);
-    const int last = min(rows - r0, 128);
+    const int last = min(rows - r0, ROWS);
     for (int r = 0; r < last; r += 8)
     {
         float2 v[8];
@@ -378,23 +407,12 @@ __global__ void __launch_bounds__(256) lce_softmax_kernel(float *z, int64_t ld, 
         *reinterpret_cast<float2 *>(colsum + blockIdx.x * ld + c) = sum;
 }
 
-__global__ void __launch_bounds__(256) lce_db_kernel(const float *__restrict__ colsum, int64_t ld, int N, const Counters *cnt, float grad_scale,
-                                                     float *__restrict__ db)
-{
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= N)
-        return;
-    const int groups = (cnt->count + 127) / 128;
-    float s          = 0.f;
-    for (int k = 0; k < groups; ++k)
-        s += colsum[k * ld + c];
-    db[c] = s * (grad_scale * cnt->inv_count);
-}
-
 // dx rows of a piece = sum of the reduction's slices, in order
 __global__ void __launch_bounds__(256) lce_slices_kernel(const float *__restrict__ part, int64_t slice, int64_t ld, int splits, int rows, int base,
                                                          const Counters *cnt, int K, const int *__restrict__ idx, float *__restrict__ dx)
 {
+    s16::let_next_in();
+    s16::after_previous();
     const int live = min(rows, cnt->count - base);
     for (int row = blockIdx.x; row < live; row += gridDim.x)
     {
@@ -409,12 +427,30 @@ __global__ void __launch_bounds__(256) lce_slices_kernel(const float *__restrict
     }
 }
 
-__global__ void __launch_bounds__(1024) lce_loss_kernel(const float *__restrict__ row_loss, const Counters *cnt, float *loss, int *err)
+// block 0: the loss, its rows added in a fixed order in double; the others: db from the column sums of the row blocks
+__global__ void __launch_bounds__(256) lce_finish_kernel(const float *__restrict__ row_loss, const float *__restrict__ colsum, int64_t ld, int rows_per_sum,
+                                                         int N, const Counters *cnt, float grad_scale, float *__restrict__ db, float *loss, int *err)
 {
-    __shared__ double box[32];
-    double s    = 0;
+    __shared__ double box[8];
+    s16::let_next_in();
+    s16::after_previous();
     const int n = cnt->count;
-    for (int i = threadIdx.x; i < n; i += 1024)
+    if (blockIdx.x > 0)
+    {
+        const int c = (blockIdx.x - 1) * 256 + threadIdx.x;
+        if (c >= N)
+            return;
+        // (pieces are multiples of the row blocks)
+        const int groups = (n + rows_per_sum - 1) / rows_per_sum;
+        float s          = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < groups; ++k)
+            s += colsum[k * ld + c];
+        db[c] = s * (grad_scale * cnt->inv_count);
+        return;
+    }
+    double s = 0;
+    for (int i = threadIdx.x; i < n; i += 256)
         s += row_loss[i];
     for (int o = 16; o > 0; o >>= 1)
         s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -423,7 +459,7 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float *__restrict_
     __syncthreads();
     if (threadIdx.x == 0)
     {
-        for (int w = 1; w < 32; ++w)
+        for (int w = 1; w < 8; ++w)
             s += box[w];
         if (loss)
             *loss = n > 0 ? static_cast<float>(s / n) : 0.f;
@@ -499,11 +535,15 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     const s16::Plan plan_x = s16::plan_tiles(R, K, N, terms, 1, true);
     const s16::Plan plan_w = out_in ? s16::plan_tiles(N, K, R, terms, 1, false) : s16::plan_tiles(K, N, R, terms, 1, false);
     const int strips       = 2 * plan_z.tiles_n(N);
+    // the softmax pass: blocks of 128 rows x 512 columns, of 32 rows where those would be fewer than the SMs
+    const int64_t sm_cols = (np + 511) / 512;
+    const int sum_rows    = (R + 127) / 128 * sm_cols < s16::sm_count() ? 32 : 128;
+    const bool own_lse    = sum_rows == 32 && sm_cols == 1;  // (a block over all columns: nobody else needs its rows' lse)
 
     const size_t scale_w = a256((N + 127) / 128 * (kp / 64) * 4), scale_x = a256(m_pad / 128 * (kp / 64) * 4);
     const size_t bytes   = 3 * a256(M * 4) + 256 + a256(N * static_cast<int64_t>(kp) * 4) + scale_w + a256(m_pad * kp * 4) + scale_x +
                          a256(static_cast<int64_t>(strips) * R * 8) + 3 * a256(piece * 4) + a256(M * 4) +
-                         (grads ? a256(piece * np * 4) : 0) + (db ? a256(m_pad / 128 * static_cast<int64_t>(np) * 4) : 0) +
+                         (grads ? a256(piece * np * 4) : 0) + (db ? a256(m_pad / sum_rows * static_cast<int64_t>(np) * 4) : 0) +
                          (dx && plan_x.splits > 1 ? a256(static_cast<int64_t>(plan_x.splits) * R * kp * 4) : 0);
     int rc = arena_begin(bytes, stream);
     if (rc)
@@ -527,20 +567,19 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     float *lse     = static_cast<float *>(take(piece * 4));
     float *picked  = static_cast<float *>(take(piece * 4));
     float *z       = grads ? static_cast<float *>(take(piece * np * 4)) : nullptr;
-    float *colsum  = db ? static_cast<float *>(take(m_pad / 128 * static_cast<int64_t>(np) * 4)) : nullptr;
+    float *colsum  = db ? static_cast<float *>(take(m_pad / sum_rows * static_cast<int64_t>(np) * 4)) : nullptr;
     float *slices  = dx && plan_x.splits > 1 ? static_cast<float *>(take(static_cast<int64_t>(plan_x.splits) * R * kp * 4)) : nullptr;
 
     lce_labels_kernel<<<1, 1024, 0, stream>>>(labels, is64, ignore_index, (int)M, (int)N, idx, cls, pos_of, cnt);
     LCE_LAUNCHED();
-    if (lse_out || dx)
     {
-        const int64_t blocks = (M + 7) / 8;
-        lce_ignored_kernel<<<(int)(blocks < 1184 ? blocks : 1184), 256, 0, stream>>>(pos_of, (int)M, (int)K, lse_out, dx);
-        LCE_LAUNCHED();
+        s16::ZeroRows zero{pos_of, dx, lse_out, (int)M, (int)K, 0};
+        if (dx || lse_out)
+            zero.blocks = (int)((M + 7) / 8 < 592 ? (M + 7) / 8 : 592);
+        if ((rc = s16::split16_encode(s16::encode_job(w, out_in ? K : N, !out_in, (int)N, (int)K, nullptr, nullptr, W, w_scale),
+                                      s16::encode_job(x, K, 0, (int)M, (int)K, idx, &cnt->count, X, x_scale), zero, stream)))
+            return rc;
     }
-    if ((rc = s16::split16_encode(w, out_in ? K : N, !out_in, (int)N, (int)K, nullptr, nullptr, W, w_scale, stream)) ||
-        (rc = s16::split16_encode(x, K, 0, (int)M, (int)K, idx, &cnt->count, X, x_scale, stream)))
-        return rc;
     gz.err = device_error_flag();
     for (int64_t base = 0; base < M; base += piece)
     {
@@ -558,13 +597,16 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
         EpiLogits::Params ez{b, cls + base, part, R, picked, z, np};
         if ((rc = gemm<true, EpiLogits>(plan_z, terms, Xp, W, g, ez, stream)))
             return rc;
-        lce_lse_kernel<<<(rows + 31) / 32, 256, 0, stream>>>(part, R, strips, rows, (int)base, cnt, idx + base, picked, lse, row_loss, lse_out);
-        LCE_LAUNCHED();
+        const LseArgs lse_args{part, R, strips, rows, (int)base, cnt, idx + base, picked, lse, row_loss, lse_out};
+        if (!(grads && own_lse) && (rc = s16::launch_after(lce_lse_kernel, dim3((rows + 31) / 32), dim3(512), 0, stream, lse_args)))
+            return rc;
         if (!grads)
             continue;
-        lce_softmax_kernel<<<dim3((rows + 127) / 128, (np + 511) / 512), 256, 0, stream>>>(
-            z, np, (int)N, (int)piece, (int)base, cnt, lse, cls + base, db ? colsum + base / 128 * static_cast<int64_t>(np) : nullptr);
-        LCE_LAUNCHED();
+        auto softmax       = sum_rows == 32 ? lce_softmax_kernel<32> : lce_softmax_kernel<128>;
+        const int row_blks = (rows + 127) / 128 * (128 / sum_rows);
+        if ((rc = s16::launch_after(softmax, dim3(row_blks, (unsigned)sm_cols), dim3(256), 0, stream, z, np, (int)N, (int)piece, lse_args, cls + base,
+                                    own_lse ? 1 : 0, db ? colsum + base / sum_rows * static_cast<int64_t>(np) : nullptr)))
+            return rc;
         Split16 P;
         P.data = reinterpret_cast<const __half *>(z);
         P.pitch = 2 * static_cast<int64_t>(np), P.rows = (int)piece, P.cols_pad = np;
@@ -578,9 +620,9 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
                 return rc;
             if (slices)
             {
-                lce_slices_kernel<<<rows < 1184 ? rows : 1184, 256, 0, stream>>>(slices, ex.slice, kp, plan_x.splits, rows, (int)base, cnt, (int)K,
-                                                                                 idx + base, dx);
-                LCE_LAUNCHED();
+                if ((rc = s16::launch_after(lce_slices_kernel, dim3(rows < 1184 ? rows : 1184), dim3(256), 0, stream, slices, ex.slice, kp, plan_x.splits,
+                                            rows, (int)base, cnt, (int)K, idx + base, dx)))
+                    return rc;
             }
         }
         if (dw)
@@ -596,13 +638,9 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
                 return rc;
         }
     }
-    if (db)
-    {
-        lce_db_kernel<<<((int)N + 255) / 256, 256, 0, stream>>>(colsum, np, (int)N, cnt, grad_scale, db);
-        LCE_LAUNCHED();
-    }
-    lce_loss_kernel<<<1, 1024, 0, stream>>>(row_loss, cnt, loss, device_error_flag());
-    LCE_LAUNCHED();
+    if ((rc = s16::launch_after(lce_finish_kernel, dim3(1 + (db ? ((int)N + 255) / 256 : 0)), dim3(256), 0, stream, row_loss, colsum, np, sum_rows, (int)N,
+                                cnt, grad_scale, db, loss, device_error_flag())))
+        return rc;
     return arena_end(stream);
 }
 

@@ -69,6 +69,7 @@ __device__ __forceinline__ float momentum_one(float &g, float &buf, float p, boo
 __global__ void __launch_bounds__(256) muon_momentum_kernel(const float *__restrict__ p, float *g, float *buf, int64_t n, MomentumArgs a, bool vec,
                                                             double *__restrict__ partial)
 {
+    s16::let_next_in();
     const int64_t off  = static_cast<int64_t>(blockIdx.y) * n;
     const bool write_g = p && (a.hook_wd > 0.f || a.grad_scale != 1.f), read_p = p && a.hook_wd > 0.f;
     double s = 0;
@@ -127,6 +128,8 @@ __global__ void __launch_bounds__(256) muon_split_kernel(const float *__restrict
                                                          __half *__restrict__ x, int64_t x_stride)
 {
     __shared__ double box[8];
+    s16::let_next_in();
+    s16::after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s       = 0;
     for (int i = threadIdx.x; i < n_partial; i += 256)
@@ -365,6 +368,8 @@ struct EpiOut
 __global__ void __launch_bounds__(256) muon_direct_kernel(const __half *__restrict__ x, int64_t x_stride, int rows, int cols, int cols_pad,
                                                           EpiOut::Params p)
 {
+    s16::let_next_in();
+    s16::after_previous();
     const int64_t n = static_cast<int64_t>(rows) * cols;
     x += blockIdx.y * x_stride;
     float *out   = p.out + blockIdx.y * p.stride;
@@ -412,16 +417,17 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
     MUON_LAUNCHED();
     int64_t sblocks = (rows * (xc / 64) + 31) / 32;
     sblocks         = sblocks > 1184 ? 1184 : sblocks;
-    muon_split_kernel<<<dim3((unsigned)sblocks, (unsigned)batch), 256, 0, stream>>>(g, buf, (int)rows, (int)cols, xc, a.momentum, a.nesterov, partial,
-                                                                                   (int)blocks, eps, x[0], x_stride);
-    MUON_LAUNCHED();
+    if ((rc = s16::launch_after(muon_split_kernel, dim3((unsigned)sblocks, (unsigned)batch), dim3(256), 0, stream, g, buf, (int)rows, (int)cols, xc, a.momentum,
+                                a.nesterov, partial, (int)blocks, eps, x[0], x_stride)))
+        return rc;
     out.ld = cols, out.stride = n;
     out.vec = !(cols & 7) && !(reinterpret_cast<uintptr_t>(out.out) & 31) && !(reinterpret_cast<uintptr_t>(out.small) & 31);
     if (steps == 0)
     {
         out.alpha = 1.f / kSx;
-        muon_direct_kernel<<<dim3((unsigned)sblocks, (unsigned)batch), 256, 0, stream>>>(x[0], x_stride, (int)rows, (int)cols, xc, out);
-        MUON_LAUNCHED();
+        if ((rc = s16::launch_after(muon_direct_kernel, dim3((unsigned)sblocks, (unsigned)batch), dim3(256), 0, stream, x[0], x_stride, (int)rows, (int)cols, xc,
+                                    out)))
+            return rc;
         return arena_end(stream);
     }
     GemmArgs gg{};
