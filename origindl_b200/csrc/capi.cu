@@ -126,15 +126,21 @@ int arena_reserve(size_t total_bytes)
     return kOk;
 }
 
-int arena_begin(size_t bytes, cudaStream_t stream)
+int check_device()
 {
     int dev = -1;
     ODL_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev != g_state.device)
-    {
-        set_last_error("the current device is %d, odl_init bound device %d", dev, g_state.device);
-        return kInvalidArgument;
-    }
+    if (dev == g_state.device)
+        return kOk;
+    set_last_error("the current device is %d, odl_init bound device %d", dev, g_state.device);
+    return kInvalidArgument;
+}
+
+int arena_begin(size_t bytes, cudaStream_t stream)
+{
+    int rc = check_device();
+    if (rc)
+        return rc;
     arena_reset();
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess)
@@ -154,7 +160,7 @@ int arena_begin(size_t bytes, cudaStream_t stream)
         g_state.recorded = true;
         return kOk;
     }
-    int rc = arena_reserve(bytes);
+    rc = arena_reserve(bytes);
     if (rc)
         return rc;
     if (g_state.last_use)

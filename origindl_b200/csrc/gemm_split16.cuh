@@ -102,6 +102,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo               = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// 32 lanes x 8 consecutive 32-bit columns of TMEM
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 // 2^x to 2^-22 of itself, 0 below the normal range
 __device__ __forceinline__ float fast_exp2(float x)
 {

@@ -19,6 +19,7 @@ void *arena_alloc(size_t bytes);
 // The arena for one call that may follow a call on another stream: resets it, makes sure `bytes` fit and orders the call
 // behind the last one that ended with arena_end.  While `stream` is being captured the block cannot grow, and one that a
 // graph has recorded is never freed.
+int check_device();  // the current device is the one odl_init bound
 int arena_begin(size_t bytes, cudaStream_t stream);
 int arena_end(cudaStream_t stream);
 // Counts replacements of library-owned scratch blocks (arena, column-sum scratch): recorded graphs compare it.

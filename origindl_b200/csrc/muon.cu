@@ -20,6 +20,7 @@
 #include "gemm_split16.cuh"
 #include "host_util.h"
 #include "internal.h"
+#include "muon.h"
 
 namespace odl
 {
@@ -30,8 +31,6 @@ using s16::GemmArgs;
 using s16::Split16;
 using s16::TileAt;
 
-constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-constexpr float kSx = 16384.f, kSa = 16384.f, kSs = 8192.f;  // halves hold value * this
 constexpr int kNormBlocks = 256;                              // at most, per matrix
 
 inline size_t a256(size_t x)
@@ -45,25 +44,6 @@ inline size_t a256(size_t x)
         ++g_launch_count;               \
         ODL_CUDA_TRY(cudaGetLastError()); \
     } while (0)
-
-struct MomentumArgs
-{
-    float momentum, hook_wd, grad_scale;
-    int nesterov;
-};
-
-// buf = momentum * buf + g, u = nesterov ? g + momentum * buf : buf (operation by operation as in the SGD step)
-__device__ __forceinline__ float momentum_one(float &g, float &buf, float p, bool has_buf, const MomentumArgs &a)
-{
-    if (a.grad_scale != 1.f)
-        g = __fmul_rn(g, a.grad_scale);
-    if (a.hook_wd > 0.f)
-        g = __fadd_rn(g, __fmul_rn(p, a.hook_wd));
-    if (!has_buf)
-        return g;
-    buf = __fadd_rn(__fmul_rn(buf, a.momentum), g);
-    return a.nesterov ? __fadd_rn(g, __fmul_rn(buf, a.momentum)) : buf;
-}
 
 // grid (blocks, batch): momentum in place and the sum of squares of u, in double (no size of gradient over- or underflows)
 __global__ void __launch_bounds__(256) muon_momentum_kernel(const float *__restrict__ p, float *g, float *buf, int64_t n, MomentumArgs a, bool vec,
@@ -303,18 +283,15 @@ struct EpiX
 // the last step's result: written out, or the parameters' update
 struct EpiOut
 {
-    struct Params
+    struct Params : NsOut
     {
-        float *out;      // result, or parameters (param != 0)
-        float *small;    // low part of the parameters
         int64_t ld, stride;
         float alpha;     // accumulator -> X
-        float keep, rate;
-        int param, vec;
+        int vec;
     };
     static __device__ __forceinline__ float one(const Params &p, float x, float was)
     {
-        return p.param ? __fsub_rn(__fmul_rn(was, p.keep), __fmul_rn(p.rate, x * p.alpha)) : x * p.alpha;
+        return ns_result(p, x * p.alpha, was);
     }
     template <int NC>
     static __device__ __forceinline__ void store(const Params &p, const GemmArgs &g, const TileAt &at, float (&v)[NC], float *slab)
@@ -399,6 +376,11 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
     const bool tall  = rows > cols;
     const int64_t m  = tall ? cols : rows;
     const int terms  = precision == ODL_PRECISION_3XTF32 ? 3 : 1;
+    if (!g_bn_override && muon_small_eligible(rows, cols, steps))
+    {
+        int rc = check_device();
+        return rc ? rc : muon_small(p, g, buf, a, out, batch, rows, cols, steps, eps, terms, stream);
+    }
     const int xc = s16::pad64(cols), mc = s16::pad64(m);
     // 256-byte multiples: rows are whole blocks of 64 columns
     const int64_t x_stride = rows * 2 * xc, m_stride = m * 2 * mc;

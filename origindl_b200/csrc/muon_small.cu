@@ -1,0 +1,555 @@
+// Newton-Schulz and the Muon step for matrices with a side of at most 128: one launch for everything.
+//
+// A matrix belongs to a cluster of 1 to 8 CTAs.  X (taken with its short side as rows) lies in their shared memory for the whole
+// iteration, split-fp16 (gemm_split16.cuh, muon.cu), each CTA holding a range of columns; nothing but the gradient, the momentum
+// and the result touches global memory.  A step in each CTA:
+//   partial A = X_loc X_loc^T      (X_loc read K-major twice; up to four accumulators, so that each sums at most two blocks of 64)
+//   A = sum over the cluster       (each CTA adds a slice of columns of all partials in rank order, and writes its halves to all)
+//   S = a I + b A + c A^2          (every CTA the whole of it: 24 MMAs, less than moving it)
+//   X_loc = S X_loc                (the same X_loc read MN-major)
+// A product of 128 x 128 takes under a microsecond here, so the steps' latencies (commit, TMEM reads, two cluster barriers)
+// bound the kernel; the form of three GEMM launches per step pays set-up, ring fill and global stores 3 * steps times instead.
+// The waits on the tensor core are bounded; one that gives up raises the error flag and the kernel runs on to its end (the cluster
+// barriers need every CTA).
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstring>
+
+#include "gemm_split16.cuh"
+#include "host_util.h"
+#include "internal.h"
+#include "muon.h"
+#include "ptx_sm100.cuh"
+
+namespace odl
+{
+
+namespace
+{
+constexpr int kThreads = 256;
+constexpr int kMaxCluster = 8;
+
+struct SmallArgs
+{
+    const float *p;
+    float *g, *buf;
+    MomentumArgs m;
+    NsOut out;
+    int *err;
+    int rows, cols;  // as stored
+    int s, l;        // short and long side
+    int s_pad;       // s rounded up to 16
+    int blocks;      // blocks of 64 columns per CTA
+    int cluster, steps, terms;
+    float eps;
+};
+
+// RB: rows of a block in shared memory (64 or 128); the MMAs' M is 128 either way, rows past RB are whatever follows (their
+// accumulator lanes are not read).  A, S and the partial A in fp32 take turns in one place: the partial sums are read before A is
+// written, and every thread writes the elements of S over the ones of A that it has just read.
+template <int RB>
+struct SmallCfg
+{
+    static constexpr int block   = RB * 128;            // bytes of 64 columns of halves
+    static constexpr int max_blk = RB == 64 ? 8 : 5;    // (TMEM holds 512 columns of X; 224 KB)
+    static constexpr int sq      = RB / 64 * block;     // bytes of an RB x RB matrix of halves
+    // X: hi blocks, lo blocks; A / S: hi, lo; the cluster's reduced slices of A (fp32)
+    __host__ __device__ static constexpr int x_lo(int blocks) { return blocks * block; }
+    __host__ __device__ static constexpr int a_hi(int blocks) { return 2 * blocks * block; }
+    __host__ __device__ static constexpr int red(int blocks) { return a_hi(blocks) + 2 * sq; }
+    // (an M = 128 read from the last RB = 64 block ends a block further on)
+    __host__ __device__ static constexpr int aux(int blocks, int cluster)
+    {
+        const int r = cluster > 1 ? 2 * sq / cluster : 0;
+        return red(blocks) + (RB == 64 && r < block ? block : r);
+    }
+    __host__ __device__ static constexpr int bytes(int blocks, int cluster) { return 1024 + aux(blocks, cluster) + 512; }
+    __host__ __device__ static constexpr bool fits(int blocks, int cluster) { return blocks <= max_blk && bytes(blocks, cluster) <= 227 * 1024; }
+};
+
+// byte of element (row, col) inside a matrix of 64-column blocks, 128-byte swizzle
+template <int RB>
+__device__ __forceinline__ uint32_t place(int row, int col)
+{
+    return static_cast<uint32_t>((col >> 6) * SmallCfg<RB>::block + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2);
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+
+template <int RB>
+__global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs p)
+{
+    using C = SmallCfg<RB>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm         = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int o_xlo = C::x_lo(p.blocks), o_ahi = C::a_hi(p.blocks), o_alo = o_ahi + C::sq, o_red = C::red(p.blocks), o_aux = C::aux(p.blocks, p.cluster);
+    uint64_t *bar       = reinterpret_cast<uint64_t *>(sm + o_aux);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 1);
+    volatile int *abort_f = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    double *box           = reinterpret_cast<double *>(sm + o_aux + 32);   // [8] warps
+    double *cl_box        = reinterpret_cast<double *>(sm + o_aux + 128);  // this CTA's sum of squares
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank   = static_cast<int>(ptx::cluster_ctarank());
+    const int matrix = blockIdx.x / p.cluster;
+    const bool tall  = p.rows > p.cols;
+    const int64_t off = static_cast<int64_t>(matrix) * p.rows * p.cols;
+    const int j0 = rank * p.blocks * 64, n_loc = p.blocks * 64;  // this CTA's columns of the wide form
+
+    if (tid == 0)
+    {
+        *abort_f = 0;
+        ptx::mbar_init(bar, 1);
+        ptx::fence_mbar_init();
+    }
+    if (warp == 0)
+    {
+        ptx::tmem_alloc(tmem_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t base = ptx::smem_u32(sm);
+
+    // ---- momentum and the norm -------------------------------------------------------------------------------------------------
+    // Elements in pairs along the long side (columns j, j + 1 of the wide form).  As stored wide: a warp covers 64 columns of a row.
+    // As stored tall: 4 short-side by 8 pairs, a compromise of 16-byte pieces of global rows and of shared-memory banks.
+    // Eight pairs at a time, so that their loads are in flight together.
+    constexpr int kBatch = 8;
+    const int n_pairs    = tall ? RB / 4 * p.blocks * 4 : RB * p.blocks;  // per lane of a warp, all warps
+    auto pair_at         = [&](int k, int &i, int &jl) {
+        if (!tall)
+            i = k % RB, jl = (k / RB) * 64 + 2 * lane;
+        else
+            i = (k % (RB / 4)) * 4 + (lane >> 3), jl = (k / (RB / 4)) * 16 + 2 * (lane & 7);
+    };
+    auto index = [&](int i, int j) -> int64_t { return off + (tall ? static_cast<int64_t>(j) * p.cols + i : static_cast<int64_t>(i) * p.cols + j); };
+    const bool write_g = p.p && (p.m.hook_wd > 0.f || p.m.grad_scale != 1.f), read_p = p.p && p.m.hook_wd > 0.f;
+    double sum         = 0;
+    constexpr int kPairs = RB * C::max_blk / (kThreads / 32);  // of a lane, at most
+    float u[kPairs][2];
+#pragma unroll
+    for (int t0 = 0; t0 < kPairs; t0 += kBatch)
+    {
+        if (warp + t0 * (kThreads / 32) >= n_pairs)
+            break;
+        float g[kBatch][2], b[kBatch][2], w[kBatch][2];
+        int64_t at[kBatch];
+        unsigned on = 0;  // bit 2 t + e: element e of pair t exists
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t)
+        {
+            const int k = warp + (t0 + t) * (kThreads / 32);
+            int i, jl;
+            pair_at(k, i, jl);
+            at[t] = index(i, j0 + jl);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                const bool in   = k < n_pairs && i < p.s && j0 + jl + e < p.l;
+                const int64_t x = at[t] + (tall ? e * p.cols : e);
+                g[t][e] = in ? p.g[x] : 0.f;
+                b[t][e] = in && p.buf ? p.buf[x] : 0.f;
+                w[t][e] = in && read_p ? p.p[x] : 0.f;
+                on |= (in ? 1u : 0u) << (2 * t + e);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                u[t0 + t][e] = momentum_one(g[t][e], b[t][e], w[t][e], p.buf != nullptr, p.m);
+                if ((on >> (2 * t + e)) & 1u)
+                {
+                    const int64_t x = at[t] + (tall ? e * p.cols : e);
+                    if (p.buf)
+                        p.buf[x] = b[t][e];
+                    if (write_g)
+                        p.g[x] = g[t][e];
+                    sum += static_cast<double>(u[t0 + t][e]) * u[t0 + t][e];
+                }
+                else
+                    u[t0 + t][e] = 0.f;
+            }
+    }
+    for (int o = 16; o > 0; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0)
+        box[warp] = sum;
+    __syncthreads();
+    if (tid == 0)
+    {
+        for (int w = 1; w < kThreads / 32; ++w)
+            sum += box[w];
+        *cl_box = sum;
+    }
+    ptx::cluster_sync();
+    double norm = 0;
+    for (int r = 0; r < p.cluster; ++r)
+    {
+        const uint32_t remote = ptx::map_to_cta(ptx::smem_u32(cl_box), r);
+        norm += __hiloint2double(static_cast<int>(ptx::ld_shared_cluster_u32(remote + 4)), static_cast<int>(ptx::ld_shared_cluster_u32(remote)));
+    }
+    norm             = sqrt(norm);
+    const double inv = static_cast<double>(kSx) / (norm > p.eps || !(norm == norm) ? norm : static_cast<double>(p.eps));
+
+    // ---- X = u / norm, in halves --------------------------------------------------------------------------------------------------
+#pragma unroll
+    for (int t = 0; t < kPairs; ++t)
+    {
+        const int k = warp + t * (kThreads / 32);
+        if (k >= n_pairs)
+            break;
+        int i, jl;
+        pair_at(k, i, jl);
+        // (an infinite norm leaves zeros where u is finite; padding stays zero whatever the norm)
+        const bool in = i < p.s;
+        uint32_t hi, lo;
+        s16::split2(in && j0 + jl < p.l ? static_cast<float>(u[t][0] * inv) : 0.f, in && j0 + jl + 1 < p.l ? static_cast<float>(u[t][1] * inv) : 0.f, hi, lo);
+        const uint32_t to                              = place<RB>(i, jl);
+        *reinterpret_cast<uint32_t *>(sm + to)         = hi;
+        *reinterpret_cast<uint32_t *>(sm + o_xlo + to) = lo;
+    }
+    ptx::fence_proxy_async_smem();
+    __syncthreads();
+
+    // ---- the iteration -----------------------------------------------------------------------------------------------------------
+    uint32_t phase = 0;
+    // descriptors: K-major with a 128-byte swizzle; X as the reduction's rows, its blocks of 64 columns C::block apart
+    auto k_major = [&](int at) { return ptx::make_smem_desc(base + at, 16, 1024, ptx::kLayoutSw128); };
+    auto rows_of_x = [&](int at) { return ptx::make_smem_desc(base + at, C::block, 1024, ptx::kLayoutSw128); };
+    // D (+)= hi hi + (lo hi + hi lo first), `n` steps of 16; step k's operands a_step(k), b_step(k) 16-byte units further
+    auto products = [&](uint32_t d, uint64_t a_hi, uint64_t a_lo, uint64_t b_hi, uint64_t b_lo, int n, auto &&a_step, auto &&b_step, uint32_t idesc, uint32_t acc) {
+        if (p.terms == 3)
+        {
+#pragma unroll 4
+            for (int k = 0; k < n; ++k)
+            {
+                s16::mma_f16(d, a_lo + a_step(k), b_hi + b_step(k), idesc, acc);
+                s16::mma_f16(d, a_hi + a_step(k), b_lo + b_step(k), idesc, 1);
+                acc = 1;
+            }
+        }
+#pragma unroll 4
+        for (int k = 0; k < n; ++k)
+        {
+            s16::mma_f16(d, a_hi + a_step(k), b_hi + b_step(k), idesc, acc);
+            acc = 1;
+        }
+    };
+    auto along_row  = [](int k) -> uint64_t { return (k >> 2) * (C::block / 16) + 2 * (k & 3); };
+    auto along_rows = [](int k) -> uint64_t { return k * (2048 / 16); };
+    auto finish_mmas = [&]() {  // all threads
+        if (!ptx::mbar_wait(bar, phase & 1, abort_f))
+            *abort_f = 1;
+        ++phase;
+        ptx::tc_fence_after_sync();
+    };
+    auto threads_meet = [&]() {
+        ptx::tc_fence_before_sync();
+        ptx::fence_proxy_async_smem();
+        __syncthreads();
+        ptx::tc_fence_after_sync();
+    };
+    const int q = warp & 3, h = warp >> 2, row = 32 * q + lane;  // drain: lane quarter, half of the columns
+    const bool mine     = 32 * q < RB;                           // (warps past RB have nothing to read)
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * q) << 16);
+    const int ksq        = p.s_pad / 16;
+    const int half_sq    = (p.s_pad / 2 + 7) / 8 * 8;            // columns of an s x s result per half
+    const int c_from = h * half_sq, c_to = h ? p.s_pad : half_sq;
+
+    for (int step = 0; step < p.steps; ++step)
+    {
+        if (tid == 0)
+        {
+            const uint32_t idesc = s16::idesc_f16(128, p.s_pad, false, false);
+            for (int b = 0; b < p.blocks; ++b)
+            {
+                const uint64_t hi = k_major(b * C::block), lo = k_major(o_xlo + b * C::block);
+                products(tmem + (b & 3) * 128, hi, lo, hi, lo, 4, along_row, along_row, idesc, b >= 4);
+            }
+            ptx::mma_commit(bar);
+        }
+        finish_mmas();
+        const int accs    = p.blocks < 4 ? p.blocks : 4;
+        constexpr float f = kSa / (kSx * kSx);
+        if (mine)
+        {
+            float *part = reinterpret_cast<float *>(sm + o_ahi);
+            for (int c = c_from; c < c_to; c += 32)
+            {
+                float v[32];
+                for (int a = 0; a < accs; ++a)
+                {
+                    uint32_t r[32];
+                    ptx::tmem_ld_32x32(lanes + a * 128 + c, r);  // (columns past c_to are other sums or unused: not written)
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        v[i] = a ? v[i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    if (c + i < c_to)
+                    {
+                        if (p.cluster == 1)
+                        {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                s16::split2(v[i + 2 * j] * f, v[i + 2 * j + 1] * f, hi[j], lo[j]);
+                            const uint32_t at                             = place<RB>(row, c + i);
+                            *reinterpret_cast<uint4 *>(sm + o_ahi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4 *>(sm + o_alo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                        else
+                        {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                part[(c + i + j) * RB + row] = v[i + j];
+                        }
+                    }
+            }
+        }
+        if (p.cluster > 1)
+        {
+            // every CTA adds up a slice of columns of all partial sums, in rank order, and all fetch all slices
+            ptx::tc_fence_before_sync();
+            ptx::cluster_sync();
+            const int slice = p.s_pad / p.cluster;
+            for (int k = tid; k < slice * (RB / 4); k += kThreads)
+            {
+                const int at = (rank * slice * RB + 4 * k) * 4;  // four rows of column rank * slice + k / (RB / 4)
+                float4 v[kMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)  // all in flight together
+                    v[r] = ld_cluster_f4(ptx::map_to_cta(base + o_ahi + at, r < p.cluster ? r : rank));
+                float4 t = v[0];
+#pragma unroll
+                for (int r = 1; r < kMaxCluster; ++r)
+                    if (r < p.cluster)
+                        t.x += v[r].x, t.y += v[r].y, t.z += v[r].z, t.w += v[r].w;
+                reinterpret_cast<float4 *>(sm + o_red)[k] = t;
+            }
+            ptx::cluster_sync();
+            // a thread: four rows of two columns; eight row groups and four column pairs a warp (shared-memory banks)
+            const int groups = RB / 32, n = p.s_pad / 8 * groups;
+            for (int k0 = warp; k0 < n; k0 += 4 * (kThreads / 32))
+            {
+                float4 v[4][2];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                {
+                    const int k = k0 + t * (kThreads / 32);
+                    const int j = k < n ? k / groups * 8 + 2 * (lane >> 3) : 0, i = k < n ? (k % groups) * 32 + 4 * (lane & 7) : 0;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        const int owner = (j + e) / slice;
+                        v[t][e]         = ld_cluster_f4(ptx::map_to_cta(base + o_red + ((j + e - owner * slice) * RB + i) * 4, owner));
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                {
+                    const int k = k0 + t * (kThreads / 32);
+                    if (k >= n)
+                        break;
+                    const int j = k / groups * 8 + 2 * (lane >> 3), i = (k % groups) * 32 + 4 * (lane & 7);
+                    const float a0[4] = {v[t][0].x, v[t][0].y, v[t][0].z, v[t][0].w}, a1[4] = {v[t][1].x, v[t][1].y, v[t][1].z, v[t][1].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        uint32_t hi, lo;
+                        s16::split2(a0[e] * f, a1[e] * f, hi, lo);
+                        const uint32_t at                                = place<RB>(i + e, j);
+                        *reinterpret_cast<uint32_t *>(sm + o_ahi + at) = hi;
+                        *reinterpret_cast<uint32_t *>(sm + o_alo + at) = lo;
+                    }
+                }
+            }
+        }
+        threads_meet();
+
+        // A^2 (A is symmetric: both operands K-major), S = a I + b A + c A^2
+        if (tid == 0)
+        {
+            products(tmem, k_major(o_ahi), k_major(o_alo), k_major(o_ahi), k_major(o_alo), ksq, along_row, along_row,
+                     s16::idesc_f16(128, p.s_pad, false, false), 0);
+            ptx::mma_commit(bar);
+        }
+        finish_mmas();
+        if (mine)
+            for (int c = c_from; c < c_to; c += 32)
+            {
+                uint32_t r[32];
+                ptx::tmem_ld_32x32(lanes + c, r);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int o = 0; o < 32; o += 8)
+                {
+                    if (c + o >= c_to)
+                        break;
+                    const uint32_t at = place<RB>(row, c + o);  // (8 columns of a row lie together)
+                    const uint4 ah = *reinterpret_cast<const uint4 *>(sm + o_ahi + at), al = *reinterpret_cast<const uint4 *>(sm + o_alo + at);
+                    const uint32_t hw[4] = {ah.x, ah.y, ah.z, ah.w}, lw[4] = {al.x, al.y, al.z, al.w};
+                    uint32_t sh[4], sl[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        const float2 fh = __half22float2(*reinterpret_cast<const __half2 *>(&hw[i])), fl = __half22float2(*reinterpret_cast<const __half2 *>(&lw[i]));
+                        float v0 = fmaf(__uint_as_float(r[o + 2 * i]), kNsC * kSs / (kSa * kSa), (fh.x + fl.x) * (kNsB * kSs / kSa));
+                        float v1 = fmaf(__uint_as_float(r[o + 2 * i + 1]), kNsC * kSs / (kSa * kSa), (fh.y + fl.y) * (kNsB * kSs / kSa));
+                        v0 += c + o + 2 * i == row && row < p.s ? kNsA * kSs : 0.f;
+                        v1 += c + o + 2 * i + 1 == row && row < p.s ? kNsA * kSs : 0.f;
+                        s16::split2(v0, v1, sh[i], sl[i]);
+                    }
+                    *reinterpret_cast<uint4 *>(sm + o_ahi + at) = make_uint4(sh[0], sh[1], sh[2], sh[3]);
+                    *reinterpret_cast<uint4 *>(sm + o_alo + at) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
+                }
+            }
+        threads_meet();
+
+        // X_loc = S X_loc
+        if (tid == 0)
+        {
+            for (int n = 0; n < n_loc; n += 256)
+            {
+                const int cols = n_loc - n < 256 ? n_loc - n : 256, at = n / 64 * C::block;
+                products(tmem + n, k_major(o_ahi), k_major(o_alo), rows_of_x(at), rows_of_x(o_xlo + at), ksq, along_row, along_rows,
+                         s16::idesc_f16(128, cols, false, true), 0);
+            }
+            ptx::mma_commit(bar);
+        }
+        finish_mmas();
+        if (mine)
+        {
+            const bool last = step + 1 == p.steps;
+            for (int c = h * (n_loc / 2); c < (h + 1) * (n_loc / 2); c += 32)
+            {
+                uint32_t r[32];
+                ptx::tmem_ld_32x32(lanes + c, r);
+                ptx::tmem_ld_wait();
+                if (!last)
+                {
+#pragma unroll
+                    for (int o = 0; o < 32; o += 8)
+                    {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s16::split2(__uint_as_float(r[o + 2 * i]) * (1.f / kSs), __uint_as_float(r[o + 2 * i + 1]) * (1.f / kSs), hi[i], lo[i]);
+                        const uint32_t at                             = place<RB>(row, c + o);
+                        *reinterpret_cast<uint4 *>(sm + at)         = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(sm + o_xlo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+                else if (row < p.s)
+                {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                    {
+                        const int j = j0 + c + i;
+                        if (j < p.l)
+                        {
+                            const int64_t k = index(row, j);
+                            const float o   = ns_result(p.out, __uint_as_float(r[i]) * (1.f / (kSs * kSx)), p.out.param ? p.out.out[k] : 0.f);
+                            p.out.out[k]    = o;
+                            if (p.out.small)
+                                p.out.small[k] = tf32_small(o);
+                        }
+                    }
+                }
+            }
+        }
+        threads_meet();
+    }
+    ptx::cluster_sync();  // nobody reads this CTA's shared memory any more
+    if (warp == 0)
+        ptx::tmem_dealloc(tmem, 512);
+    if (tid == 0 && *abort_f)
+        atomicExch(p.err, 1);
+}
+}  // namespace
+
+namespace
+{
+// CTAs of a matrix: as few as hold X; more, down to two blocks each, while the GPU has SMs for them.  0: it does not fit.
+template <int RB>
+int cluster_for(int blocks, int64_t batch)
+{
+    using C = SmallCfg<RB>;
+    int c   = 1;
+    while (c <= kMaxCluster && !C::fits((blocks + c - 1) / c, c))
+        c *= 2;
+    if (c > kMaxCluster)
+        return 0;
+    while (c < kMaxCluster && blocks >= 4 * c && 2 * c * batch <= s16::sm_count() && C::fits((blocks + 2 * c - 1) / (2 * c), 2 * c))
+        c *= 2;
+    return c;
+}
+}  // namespace
+
+bool muon_small_eligible(int64_t rows, int64_t cols, int steps)
+{
+    const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+    if (steps <= 0 || s > 128 || l > 64 * SmallCfg<64>::max_blk * kMaxCluster)
+        return false;
+    const int blocks = static_cast<int>((l + 63) / 64);
+    return (s <= 64 ? cluster_for<64>(blocks, 1 << 20) : cluster_for<128>(blocks, 1 << 20)) > 0;
+}
+
+int muon_small(const float *p, float *g, float *buf, const MomentumArgs &a, const NsOut &out, int64_t batch, int64_t rows, int64_t cols, int steps,
+               float eps, int terms, cudaStream_t stream)
+{
+    SmallArgs k{};
+    k.p = p, k.g = g, k.buf = buf, k.m = a, k.out = out, k.err = device_error_flag();
+    k.rows = (int)rows, k.cols = (int)cols;
+    k.s = (int)(rows < cols ? rows : cols), k.l = (int)(rows < cols ? cols : rows);
+    k.s_pad = (k.s + 15) / 16 * 16;
+    k.steps = steps, k.terms = terms, k.eps = eps;
+    const bool narrow = k.s <= 64;
+    const int all     = (k.l + 63) / 64;
+    const int c       = narrow ? cluster_for<64>(all, batch) : cluster_for<128>(all, batch);
+    k.cluster = c;
+    k.blocks  = (all + c - 1) / c;
+    auto kernel    = narrow ? muon_small_kernel<64> : muon_small_kernel<128>;
+    const int smem = narrow ? SmallCfg<64>::bytes(k.blocks, c) : SmallCfg<128>::bytes(k.blocks, c);
+    static bool set[2] = {false, false};
+    if (!set[narrow])
+    {
+        ODL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        set[narrow] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim          = dim3(static_cast<unsigned>(batch * c));
+    cfg.blockDim         = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream           = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id               = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs                = attr;
+    cfg.numAttrs             = 1;
+    cudaError_t e            = cudaLaunchKernelEx(&cfg, kernel, k);
+    ++g_launch_count;
+    if (e != cudaSuccess)
+    {
+        set_last_error("muon_small_kernel launch failed: %s", cudaGetErrorString(e));
+        return kCudaError;
+    }
+    return kOk;
+}
+
+}  // namespace odl

@@ -63,7 +63,7 @@ def bound(g, steps, precision):
     return want, 4 * far
 
 
-SHAPES = [(1, 1), (1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (63, 200), (128, 128), (129, 127), (100, 784), (784, 100),
+SHAPES = [(16, 700), (700, 16), (64, 4096), (64, 4097), (4000, 60), (128, 1536), (128, 1537), (1500, 120), (65, 1000), (100, 2000), (8, 64), (1, 1), (1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (63, 200), (128, 128), (129, 127), (100, 784), (784, 100),
           (256, 256), (257, 300), (300, 257), (513, 1000), (1000, 513), (1024, 384), (1100, 1100), (260, 2000)]
 
 
@@ -118,7 +118,7 @@ def test_plain_tf32(ops, rows, cols):
     assert torch.linalg.matrix_norm(got.double() - want).item() <= far
 
 
-@pytest.mark.parametrize("batch,rows,cols", [(3, 50, 70), (5, 130, 64), (2, 257, 513), (33, 16, 24), (4, 600, 300)])
+@pytest.mark.parametrize("batch,rows,cols", [(40, 64, 512), (150, 9, 40), (300, 32, 130), (20, 500, 100), (3, 50, 70), (5, 130, 64), (2, 257, 513), (33, 16, 24), (4, 600, 300)])
 def test_stack(ops, batch, rows, cols):
     g = gradient(batch, rows, cols, seed=batch)
     g[1] *= 1e-3   # each has its own norm
