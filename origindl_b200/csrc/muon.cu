@@ -56,36 +56,49 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const float *__restr
     g += off;
     buf = buf ? buf + off : nullptr;
     p   = p ? p + off : nullptr;
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-    int64_t i            = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (vec)
+    // four values at a time, whatever the alignment (the sum has the same bits)
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * 256, n4 = (n + 3) >> 2;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n4; i += stride)
     {
-        const int64_t n4 = n >> 2;
-        for (; i < n4; i += stride)
-        {
-            float4 G = reinterpret_cast<const float4 *>(g)[i];
-            float4 M = buf ? reinterpret_cast<const float4 *>(buf)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 P = read_p ? reinterpret_cast<const float4 *>(p)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float u0 = momentum_one(G.x, M.x, P.x, buf, a), u1 = momentum_one(G.y, M.y, P.y, buf, a);
-            const float u2 = momentum_one(G.z, M.z, P.z, buf, a), u3 = momentum_one(G.w, M.w, P.w, buf, a);
-            if (buf)
-                reinterpret_cast<float4 *>(buf)[i] = M;
-            if (write_g)
-                reinterpret_cast<float4 *>(g)[i] = G;
-            s += static_cast<double>(u0) * u0 + static_cast<double>(u1) * u1;
-            s += static_cast<double>(u2) * u2 + static_cast<double>(u3) * u3;
-        }
-        i = (n4 << 2) + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    }
-    for (; i < n; i += stride)
-    {
-        float G = g[i], M = buf ? buf[i] : 0.f;
-        const float u = momentum_one(G, M, read_p ? p[i] : 0.f, buf, a);
+        float G[4], M[4] = {0.f, 0.f, 0.f, 0.f}, P[4] = {0.f, 0.f, 0.f, 0.f}, u[4];
+        const int have = n - 4 * i < 4 ? static_cast<int>(n - 4 * i) : 4;
+        auto load      = [&](const float *src, float (&v)[4]) {
+            if (vec)
+            {
+                const float4 q = reinterpret_cast<const float4 *>(src)[i];
+                v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[j] = j < have ? src[4 * i + j] : 0.f;
+            }
+        };
+        auto store = [&](float *dst, const float (&v)[4]) {
+            if (vec)
+                reinterpret_cast<float4 *>(dst)[i] = make_float4(v[0], v[1], v[2], v[3]);
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < have)
+                        dst[4 * i + j] = v[j];
+            }
+        };
+        load(g, G);
         if (buf)
-            buf[i] = M;
+            load(buf, M);
+        if (read_p)
+            load(p, P);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            u[j] = momentum_one(G[j], M[j], P[j], buf, a);
+        if (buf)
+            store(buf, M);
         if (write_g)
-            g[i] = G;
-        s += static_cast<double>(u) * u;
+            store(g, G);
+        s += square_sum(u);
     }
     __shared__ double box[8];
     for (int o = 16; o > 0; o >>= 1)
@@ -119,12 +132,11 @@ __global__ void __launch_bounds__(256) muon_split_kernel(const float *__restrict
     if (lane == 0)
         box[warp] = s;
     __syncthreads();
-    // the factor in double: 1 / norm of a tiny or huge gradient need not be a float
     double norm = 0;
     for (int w = 0; w < 8; ++w)
         norm += box[w];
     norm             = sqrt(norm);
-    const double inv = static_cast<double>(kSx) / (norm > eps || !(norm == norm) ? norm : static_cast<double>(eps));
+    const InverseNorm inv = inverse_norm(norm, eps, kSx);
     const int64_t off = static_cast<int64_t>(blockIdx.y) * rows * cols;
     const int blocks  = cols_pad / 64;
     const int64_t all = static_cast<int64_t>(rows) * blocks;
@@ -144,7 +156,7 @@ __global__ void __launch_bounds__(256) muon_split_kernel(const float *__restrict
                 v[j]             = !buf ? g[at] : nesterov ? __fadd_rn(g[at], __fmul_rn(m, momentum)) : m;
             }
         uint32_t hi, lo;
-        s16::split2(static_cast<float>(v[0] * inv), static_cast<float>(v[1] * inv), hi, lo);
+        s16::split2(inv.times(v[0]), inv.times(v[1]), hi, lo);
         out[k * 64 + lane]      = hi;
         out[k * 64 + 32 + lane] = lo;
     }

@@ -15,6 +15,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "gemm_split16.cuh"
 #include "host_util.h"
@@ -119,67 +120,103 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
     const uint32_t base = ptx::smem_u32(sm);
 
     // ---- momentum and the norm -------------------------------------------------------------------------------------------------
-    // Elements in pairs along the long side (columns j, j + 1 of the wide form).  As stored wide: a warp covers 64 columns of a row.
-    // As stored tall: 4 short-side by 8 pairs, a compromise of 16-byte pieces of global rows and of shared-memory banks.
-    // Eight pairs at a time, so that their loads are in flight together.
-    constexpr int kBatch = 8;
-    const int n_pairs    = tall ? RB / 4 * p.blocks * 4 : RB * p.blocks;  // per lane of a warp, all warps
-    auto pair_at         = [&](int k, int &i, int &jl) {
+    // A thread's elements come in pairs along the long side (columns j, j + 1 of the wide form), N pairs at a time, their loads
+    // unconditional (from the matrix's first element where there is nothing) so that they are in flight together.  As stored wide
+    // a warp covers 64 columns of a row, a batch 8 rows; as stored tall a warp covers 4 short-side by 8 pairs (a compromise of
+    // 16-byte pieces of global rows and of shared-memory banks), a batch 64 columns.
+    auto batches = [&](auto &&body) {
         if (!tall)
-            i = k % RB, jl = (k / RB) * 64 + 2 * lane;
-        else
-            i = (k % (RB / 4)) * 4 + (lane >> 3), jl = (k / (RB / 4)) * 16 + 2 * (lane & 7);
-    };
-    auto index = [&](int i, int j) -> int64_t { return off + (tall ? static_cast<int64_t>(j) * p.cols + i : static_cast<int64_t>(i) * p.cols + j); };
-    const bool write_g = p.p && (p.m.hook_wd > 0.f || p.m.grad_scale != 1.f), read_p = p.p && p.m.hook_wd > 0.f;
-    double sum         = 0;
-    constexpr int kPairs = RB * C::max_blk / (kThreads / 32);  // of a lane, at most
-    float u[kPairs][2];
-#pragma unroll
-    for (int t0 = 0; t0 < kPairs; t0 += kBatch)
-    {
-        if (warp + t0 * (kThreads / 32) >= n_pairs)
-            break;
-        float g[kBatch][2], b[kBatch][2], w[kBatch][2];
-        int64_t at[kBatch];
-        unsigned on = 0;  // bit 2 t + e: element e of pair t exists
-#pragma unroll
-        for (int t = 0; t < kBatch; ++t)
         {
-            const int k = warp + (t0 + t) * (kThreads / 32);
-            int i, jl;
-            pair_at(k, i, jl);
-            at[t] = index(i, j0 + jl);
+#pragma unroll 1
+            for (int b = 0; b < p.blocks; ++b)
+#pragma unroll 1
+                for (int i = warp; i < RB; i += 64)
+                    body(std::integral_constant<bool, false>(), std::integral_constant<int, 8>(), i, 64 * b + 2 * lane);
+        }
+        else
+        {
+#pragma unroll 1
+            for (int i = 4 * warp + (lane >> 3); i < RB; i += 32)
+#pragma unroll 1
+                for (int c = 0; c < n_loc; c += 64)
+                    body(std::integral_constant<bool, true>(), std::integral_constant<int, 4>(), i, c + 2 * (lane & 7));
+        }
+    };
+    // pair t of a batch: row, column of this CTA, and the places of its elements in the matrix (-1: there is none; a matrix has
+    // under 2^31 elements here)
+    struct Pair
+    {
+        int i, c, x0, x1;
+    };
+    auto pair = [&](auto is_tall, int t, int i, int c) -> Pair {
+        constexpr bool T = decltype(is_tall)::value;
+        Pair q;
+        q.i = T ? i : i + 8 * t, q.c = T ? c + 16 * t : c;
+        const int j = j0 + q.c, x = T ? j * p.cols + q.i : q.i * p.cols + j;
+        q.x0 = q.i < p.s && j < p.l ? x : -1;
+        q.x1 = q.i < p.s && j + 1 < p.l ? x + (T ? p.cols : 1) : -1;
+        return q;
+    };
+    const bool write_g = p.p && (p.m.hook_wd > 0.f || p.m.grad_scale != 1.f), read_p = p.p && p.m.hook_wd > 0.f;
+    float *const G = p.g + off, *const B = p.buf ? p.buf + off : nullptr;
+    const float *const P = read_p ? p.p + off : nullptr;
+    // both elements of a pair as one 8-byte access (both or none exist: cols is even)
+    auto even      = [&](const float *q) { return !(reinterpret_cast<uintptr_t>(q) & 7); };
+    const bool two = !tall && !(p.cols & 1) && even(G) && even(B) && even(P);
+    auto load_pair = [&](const float *src, const Pair &q, bool both, float (&v)[2]) {
+        const int y0 = q.x0 < 0 ? 0 : q.x0, y1 = q.x1 < 0 ? 0 : q.x1;
+        if (both)
+        {
+            const float2 f = *reinterpret_cast<const float2 *>(src + y0);
+            v[0] = f.x, v[1] = f.y;
+        }
+        else
+            v[0] = src[y0], v[1] = src[y1];
+    };
+    auto store_pair = [&](float *dst, const Pair &q, bool both, float v0, float v1) {
+        if (both)
+        {
+            if (q.x0 >= 0)
+                *reinterpret_cast<float2 *>(dst + q.x0) = make_float2(v0, v1);
+            return;
+        }
+        if (q.x0 >= 0)
+            dst[q.x0] = v0;
+        if (q.x1 >= 0)
+            dst[q.x1] = v1;
+    };
+    double sum = 0;
+    batches([&](auto is_tall, auto n, int i, int c) {
+        constexpr int N = decltype(n)::value;
+        float g[N][2], b[N][2], w[N][2], u[2 * N];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-                const bool in   = k < n_pairs && i < p.s && j0 + jl + e < p.l;
-                const int64_t x = at[t] + (tall ? e * p.cols : e);
-                g[t][e] = in ? p.g[x] : 0.f;
-                b[t][e] = in && p.buf ? p.buf[x] : 0.f;
-                w[t][e] = in && read_p ? p.p[x] : 0.f;
-                on |= (in ? 1u : 0u) << (2 * t + e);
-            }
+        for (int t = 0; t < N; ++t)
+        {
+            const Pair q = pair(is_tall, t, i, c);
+            load_pair(G, q, two, g[t]);
+            b[t][0] = b[t][1] = w[t][0] = w[t][1] = 0.f;
+            if (B)
+                load_pair(B, q, two, b[t]);
+            if (P)
+                load_pair(P, q, two, w[t]);
         }
 #pragma unroll
-        for (int t = 0; t < kBatch; ++t)
+        for (int t = 0; t < N; ++t)
+        {
+            const Pair q = pair(is_tall, t, i, c);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
             {
-                u[t0 + t][e] = momentum_one(g[t][e], b[t][e], w[t][e], p.buf != nullptr, p.m);
-                if ((on >> (2 * t + e)) & 1u)
-                {
-                    const int64_t x = at[t] + (tall ? e * p.cols : e);
-                    if (p.buf)
-                        p.buf[x] = b[t][e];
-                    if (write_g)
-                        p.g[x] = g[t][e];
-                    sum += static_cast<double>(u[t0 + t][e]) * u[t0 + t][e];
-                }
-                else
-                    u[t0 + t][e] = 0.f;
+                const float v = momentum_one(g[t][e], b[t][e], w[t][e], B != nullptr, p.m);
+                u[2 * t + e]  = (e ? q.x1 : q.x0) >= 0 ? v : 0.f;
             }
-    }
+            if (B)
+                store_pair(B, q, two, b[t][0], b[t][1]);
+            if (write_g)
+                store_pair(G, q, two, g[t][0], g[t][1]);
+        }
+        sum += square_sum(u);
+    });
     for (int o = 16; o > 0; o >>= 1)
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0)
@@ -199,25 +236,40 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
         norm += __hiloint2double(static_cast<int>(ptx::ld_shared_cluster_u32(remote + 4)), static_cast<int>(ptx::ld_shared_cluster_u32(remote)));
     }
     norm             = sqrt(norm);
-    const double inv = static_cast<double>(kSx) / (norm > p.eps || !(norm == norm) ? norm : static_cast<double>(p.eps));
+    const InverseNorm inv = inverse_norm(norm, p.eps, kSx);
 
-    // ---- X = u / norm, in halves --------------------------------------------------------------------------------------------------
+    // ---- X = u / norm, in halves (u formed again by the thread that formed it: the same operations, the same bits) -----------------
+    batches([&](auto is_tall, auto n, int i, int c) {
+        constexpr int N = decltype(n)::value;
+        float g[N][2], b[N][2];
 #pragma unroll
-    for (int t = 0; t < kPairs; ++t)
-    {
-        const int k = warp + t * (kThreads / 32);
-        if (k >= n_pairs)
-            break;
-        int i, jl;
-        pair_at(k, i, jl);
-        // (an infinite norm leaves zeros where u is finite; padding stays zero whatever the norm)
-        const bool in = i < p.s;
-        uint32_t hi, lo;
-        s16::split2(in && j0 + jl < p.l ? static_cast<float>(u[t][0] * inv) : 0.f, in && j0 + jl + 1 < p.l ? static_cast<float>(u[t][1] * inv) : 0.f, hi, lo);
-        const uint32_t to                              = place<RB>(i, jl);
-        *reinterpret_cast<uint32_t *>(sm + to)         = hi;
-        *reinterpret_cast<uint32_t *>(sm + o_xlo + to) = lo;
-    }
+        for (int t = 0; t < N; ++t)
+        {
+            const Pair q = pair(is_tall, t, i, c);
+            g[t][0] = g[t][1] = b[t][0] = b[t][1] = 0.f;
+            if (!B || p.m.nesterov)
+                load_pair(G, q, two, g[t]);
+            if (B)
+                load_pair(B, q, two, b[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+        {
+            const Pair q = pair(is_tall, t, i, c);
+            float v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                const float u = !B ? g[t][e] : p.m.nesterov ? __fadd_rn(g[t][e], __fmul_rn(b[t][e], p.m.momentum)) : b[t][e];
+                v[e]          = (e ? q.x1 : q.x0) >= 0 ? inv.times(u) : 0.f;
+            }
+            uint32_t hi, lo;
+            s16::split2(v[0], v[1], hi, lo);
+            const uint32_t to                              = place<RB>(q.i, q.c);
+            *reinterpret_cast<uint32_t *>(sm + to)         = hi;
+            *reinterpret_cast<uint32_t *>(sm + o_xlo + to) = lo;
+        }
+    });
     ptx::fence_proxy_async_smem();
     __syncthreads();
 
@@ -280,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
         }
         finish_mmas();
         const int accs    = p.blocks < 4 ? p.blocks : 4;
-        constexpr float f = kSa / (kSx * kSx);
+        constexpr float f = kSa / (kSx * kSx), f_out = 1.f / (kSs * kSx);
         if (mine)
         {
             float *part = reinterpret_cast<float *>(sm + o_ahi);
@@ -452,26 +504,43 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
                         *reinterpret_cast<uint4 *>(sm + o_xlo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
-                else if (row < p.s)
+                else
                 {
+                    // the result in fp32, 256 bytes a row of a block, over X (dead); 16-byte pieces change places by the row
+                    float4 *to = reinterpret_cast<float4 *>(sm + ((c >> 6) * RB + row) * 256);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                    {
-                        const int j = j0 + c + i;
-                        if (j < p.l)
-                        {
-                            const int64_t k = index(row, j);
-                            const float o   = ns_result(p.out, __uint_as_float(r[i]) * (1.f / (kSs * kSx)), p.out.param ? p.out.out[k] : 0.f);
-                            p.out.out[k]    = o;
-                            if (p.out.small)
-                                p.out.small[k] = tf32_small(o);
-                        }
-                    }
+                    for (int o = 0; o < 32; o += 4)
+                        to[(((c & 32) + o) >> 2) ^ (row & 15)] = make_float4(__uint_as_float(r[o]) * f_out, __uint_as_float(r[o + 1]) * f_out,
+                                                                           __uint_as_float(r[o + 2]) * f_out, __uint_as_float(r[o + 3]) * f_out);
                 }
             }
         }
         threads_meet();
     }
+    // ---- the result, by the threads and in the order that read the gradient --------------------------------------------------------
+    float *const O = p.out.out + off, *const L = p.out.small ? p.out.small + off : nullptr;
+    const bool two_out = !tall && !(p.cols & 1) && even(O) && even(L);
+    batches([&](auto is_tall, auto n, int i, int c) {
+        constexpr int N = decltype(n)::value;
+        float was[N][2];
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+        {
+            was[t][0] = was[t][1] = 0.f;
+            if (p.out.param)
+                load_pair(O, pair(is_tall, t, i, c), two_out, was[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+        {
+            const Pair q   = pair(is_tall, t, i, c);
+            const float2 x = *reinterpret_cast<const float2 *>(sm + ((q.c >> 6) * RB + q.i) * 256 + ((((q.c & 63) >> 2) ^ (q.i & 15)) << 4) + (q.c & 2) * 4);
+            const float o0 = ns_result(p.out, x.x, was[t][0]), o1 = ns_result(p.out, x.y, was[t][1]);
+            store_pair(O, q, two_out, o0, o1);
+            if (L)
+                store_pair(L, q, two_out, tf32_small(o0), tf32_small(o1));
+        }
+    });
     ptx::cluster_sync();  // nobody reads this CTA's shared memory any more
     if (warp == 0)
         ptx::tmem_dealloc(tmem, 512);
