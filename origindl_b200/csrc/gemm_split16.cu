@@ -110,55 +110,65 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_
 
 namespace
 {
-// One 128 x 64 tile per block: read once, its largest finite value gives the tile's power of two, written as halves.
-// Bound by memory: 4 bytes in and 4 out per value.  A launch holds two matrices (x and W of a loss) and a range of blocks that
-// put zeros into rows of `zero` and words of `zero_lse` (rows without a label: pos_of < 0).
-__device__ __forceinline__ void split16_tile(const EncodeJob &j, int block, float (&box)[8], float (&tile)[64][129])
+// One 128 x 128 tile per block of 512 threads: read once, its largest finite value gives the tile's power of two, written as
+// halves.  Bound by memory: 4 bytes in and 4 out per value.  A launch holds two matrices (x and W of a loss) and a range of blocks
+// that put zeros into rows of `zero` (rows without a label: pos_of < 0).
+constexpr int kTileThreads = 512;
+
+__device__ __forceinline__ void split16_tile(const EncodeJob &j, int block, float (&box)[16], float (&tile)[64][129])
 {
     // neighbouring blocks take neighbouring columns: rows are read in long stretches
     const int block_c = block % j.blocks_c, block_r = block / j.blocks_c;
-    const int c0 = block_c * 64, r0 = block_r * 128;
+    const int c0 = block_c * 128, r0 = block_r * 128;
     const int live = j.count ? min(j.rows, *j.count) : j.rows;
     if (r0 >= live)
         return;  // (gathered matrices: nobody reads rows past the last 128 that hold any)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // thread: rows (lane / 16) + 2 warp + 16 i, columns 4 (lane % 16) .. + 3 of the tile
-    const int cc = 4 * (lane & 15), rr = 2 * warp + (lane >> 4);
+    const int c = c0 + 4 * lane;  // thread: columns c .. c + 3 of rows warp + 16 i
     float4 v[8];
     if (j.transposed)
     {
         const bool vec = !(j.ld & 3) && !(reinterpret_cast<uintptr_t>(j.src) & 15) && r0 + 128 <= live;
-        for (int i = warp; i < 64; i += 8)
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h)  // 64 columns at a time through shared memory
         {
-            const float *line = j.src + (c0 + i) * j.ld + r0;
-            if (vec && c0 + i < j.cols)
+            __syncthreads();
+            for (int i = warp; i < 64; i += 16)
             {
-                const float4 q = __ldg(reinterpret_cast<const float4 *>(line) + lane);
-                tile[i][4 * lane] = q.x, tile[i][4 * lane + 1] = q.y, tile[i][4 * lane + 2] = q.z, tile[i][4 * lane + 3] = q.w;
-            }
-            else
-                for (int k = 0; k < 4; ++k)
+                const int col     = c0 + 64 * h + i;
+                const float *line = j.src + col * j.ld + r0;
+                if (vec && col < j.cols)
                 {
-                    const int r = lane + 32 * k;
-                    tile[i][r]  = (c0 + i < j.cols && r0 + r < live) ? __ldg(line + r) : 0.f;
+                    const float4 q = __ldg(reinterpret_cast<const float4 *>(line) + lane);
+                    tile[i][4 * lane] = q.x, tile[i][4 * lane + 1] = q.y, tile[i][4 * lane + 2] = q.z, tile[i][4 * lane + 3] = q.w;
                 }
-        }
-        __syncthreads();
+                else
+                    for (int k = 0; k < 4; ++k)
+                    {
+                        const int r = lane + 32 * k;
+                        tile[i][r]  = (col < j.cols && r0 + r < live) ? __ldg(line + r) : 0.f;
+                    }
+            }
+            __syncthreads();
+            if ((lane >> 4) == h)
+            {
+                const int cc = 4 * (lane & 15);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-        {
-            const int r = rr + 16 * i;
-            v[i]        = make_float4(tile[cc][r], tile[cc + 1][r], tile[cc + 2][r], tile[cc + 3][r]);
+                for (int i = 0; i < 8; ++i)
+                {
+                    const int r = warp + 16 * i;
+                    v[i]        = make_float4(tile[cc][r], tile[cc + 1][r], tile[cc + 2][r], tile[cc + 3][r]);
+                }
+            }
         }
     }
     else
     {
-        const int c    = c0 + cc;
         const bool vec = !(j.ld & 3) && !(j.cols & 3) && !(reinterpret_cast<uintptr_t>(j.src) & 15);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
         {
-            const int r = r0 + rr + 16 * i;
+            const int r = r0 + warp + 16 * i;
             v[i]        = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < live)
             {
@@ -198,7 +208,7 @@ __device__ __forceinline__ void split16_tile(const EncodeJob &j, int block, floa
         box[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w)
+    for (int w = 0; w < 16; ++w)
         top = fmaxf(top, box[w]);
     // s = 2^(e - 14) with 2^e <= top < 2^(e + 1): v / s below 2^15, fp16's largest is just under 2^16
     const int e     = top > 0.f ? max(ilogbf(top), -112) : 0;
@@ -206,25 +216,27 @@ __device__ __forceinline__ void split16_tile(const EncodeJob &j, int block, floa
     const float inv = __int_as_float((127 - (e - 14)) << 23);
     if (threadIdx.x == 0)
         j.scale[block] = s;
+    if (c >= j.cols_pad)
+        return;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
     {
-        const int r = r0 + rr + 16 * i;
+        const int r = r0 + warp + 16 * i;
         if (r < (j.gather ? r0 + 128 : j.rows))
         {
             uint2 hi, lo;
             split2(v[i].x * inv, v[i].y * inv, hi.x, lo.x);
             split2(v[i].z * inv, v[i].w * inv, hi.y, lo.y);
-            __half *line = j.out + r * j.pitch + 2 * c0 + cc;
+            __half *line = j.out + r * j.pitch + (c >> 6) * 128 + (c & 63);
             *reinterpret_cast<uint2 *>(line)      = hi;
             *reinterpret_cast<uint2 *>(line + 64) = lo;
         }
     }
 }
 
-__global__ void __launch_bounds__(256) split16_tiles_kernel(const __grid_constant__ EncodeJob a, const __grid_constant__ EncodeJob b, const ZeroRows z)
+__global__ void __launch_bounds__(kTileThreads) split16_tiles_kernel(const __grid_constant__ EncodeJob a, const __grid_constant__ EncodeJob b, const ZeroRows z)
 {
-    __shared__ float box[8];
+    __shared__ float box[16];
     __shared__ float tile[64][129];
     let_next_in();
     after_previous();
@@ -236,7 +248,8 @@ __global__ void __launch_bounds__(256) split16_tiles_kernel(const __grid_constan
         return split16_tile(b, block, box, tile);
     block -= b.blocks;
     const int lane = threadIdx.x & 31;
-    for (int row = block * 8 + (threadIdx.x >> 5); row < z.rows; row += z.blocks * 8)
+    constexpr int kWarps = kTileThreads / 32;
+    for (int row = block * kWarps + (threadIdx.x >> 5); row < z.rows; row += z.blocks * kWarps)
     {
         if (z.pos_of[row] >= 0)
             continue;
@@ -254,7 +267,8 @@ EncodeJob encode_job(const float *src, int64_t ld, int transposed, int rows, int
     EncodeJob j;
     j.src = src, j.ld = ld, j.transposed = transposed, j.rows = rows, j.cols = cols, j.gather = gather, j.count = count;
     j.out = const_cast<__half *>(out.data), j.pitch = out.pitch, j.scale = scale;
-    j.blocks_c = out.cols_pad / 64;
+    j.cols_pad = out.cols_pad;
+    j.blocks_c = (out.cols_pad + 127) / 128;
     j.blocks   = static_cast<int64_t>((rows + 127) / 128) * j.blocks_c;
     return j;
 }
@@ -267,7 +281,7 @@ int split16_encode(const EncodeJob &a, const EncodeJob &b, const ZeroRows &z, cu
         set_last_error("split: %lld tiles are too many", (long long)blocks);
         return kTooLarge;
     }
-    return launch_after(split16_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, b, z);
+    return launch_after(split16_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0, stream, a, b, z);
 }
 
 }  // namespace s16

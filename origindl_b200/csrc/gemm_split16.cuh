@@ -3,7 +3,7 @@
 // two such matrices is three fp16 products, hi hi + lo hi + hi lo (the dropped lo lo is at most 2^-22), with fp32
 // accumulation: the accuracy of the 3xTF32 GEMM at twice its rate, since tcgen05 multiplies fp16 twice as fast as tf32 and
 // both have 11-bit significands.  fp16's short exponent is what s is for: an operand has one s for all of it (Newton-Schulz
-// iterates, whose entries are bounded; softmax probabilities) or one for each 128 x 64 tile (see Split16 below).
+// iterates, whose entries are bounded; softmax probabilities) or one for each 128 x 128 tile (see Split16 below).
 //
 // Layout of a split matrix of R rows and C columns (C padded to a multiple of 64 with zeros): row after row, and within a
 // row, block of 64 columns after block, [64 hi][64 lo]: 256 bytes, exactly the bytes of the 64 fp32 values, so that a matrix
@@ -11,9 +11,11 @@
 //
 // The kernel: persistent, one CTA (128 x BN tiles) or a CTA pair (256 x 256, tcgen05 cta_group::2) per SM (pair), warp 0 feeds a
 // ring of 64-deep K-blocks by TMA (no multicast), one thread of warp 1 issues the MMAs, eight warps drain the accumulator.
-// TMEM accumulation truncates (a step of the accumulator per instruction), so an accumulator holds one K-block only: two TMEM
-// buffers alternate, and the drain adds them up in fp32 registers, scaled by the tiles' s where the operands have many.  The
-// small products go first, so that only four instructions truncate at full size.
+// TMEM accumulation truncates (a step of the accumulator per instruction), so an accumulator holds 128 of the reduction only: two
+// TMEM buffers alternate, and the drain adds them up in fp32 registers, scaled by the tiles' s where the operands have many.  Of
+// each K-block the small products go first, so that only four instructions truncate at full size.  The epilogue holds up the
+// drain (8 to 18 thousand cycles a tile, when all SMs store at once, against 1536 a K-block); the MMA thread runs two buffers
+// ahead of it, and where no scales are in the way the first two buffers of a tile take 256 of the reduction each.
 // Every wait is bounded; a wait that gives up raises the abort flag, which releases the others, and the error flag.
 #pragma once
 #include <cuda.h>
@@ -47,7 +49,7 @@ struct Split16
     int rows = 0, cols_pad = 0;
     int batch            = 1;
     int64_t batch_stride = 0;      // halves
-    const float *scale   = nullptr;  // s of each 128 x 64 tile, [ceil(rows / 128)][cols_pad / 64]; nullptr: one s, in `alpha`
+    const float *scale   = nullptr;  // s of each 128 x 128 tile, [ceil(rows / 128)][ceil(cols_pad / 128)]; nullptr: one s, in `alpha`
 };
 
 inline int pad64(int64_t c)
@@ -144,6 +146,13 @@ struct Cfg
     static constexpr int strip   = BN / 2;  // columns of the tile one epilogue warp holds
 };
 
+// K-blocks of a tile's c-th chunk (what one accumulator buffer holds); 128 of the reduction is also what a tile scale covers
+template <bool SCALED>
+__device__ __forceinline__ int chunk_blocks(int c)
+{
+    return SCALED || c >= 2 ? 2 : 4;
+}
+
 // what the epilogue is told about a tile
 struct TileAt
 {
@@ -165,8 +174,9 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
     uint8_t *tiles      = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *slabs        = reinterpret_cast<float *>(tiles + C::stages * C::stage);
     uint64_t *full_bar  = reinterpret_cast<uint64_t *>(tiles + C::stages * C::stage + kEpi * kSlab);
-    uint64_t *done_bar  = full_bar + C::stages;  // a stage's MMAs are complete: its buffers are free, its accumulator is full
-    uint64_t *acc_empty = done_bar + C::stages;
+    uint64_t *empty_bar = full_bar + C::stages;  // a stage's MMAs are complete: its buffers are free
+    uint64_t *acc_full  = empty_bar + C::stages;
+    uint64_t *acc_empty = acc_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     volatile int *abort_f = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *early_out        = const_cast<int *>(abort_f) + 1;
@@ -183,10 +193,13 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
         for (int s = 0; s < C::stages; ++s)
         {
             ptx::mbar_init(&full_bar[s], 1);
-            ptx::mbar_init(&done_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b)
+        {
+            ptx::mbar_init(&acc_full[b], 1);
             ptx::mbar_init(&acc_empty[b], CG * kEpi);
+        }
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm.a);
         ptx::prefetch_tmap(&tm.b);
@@ -228,14 +241,23 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
     // (a later piece of the reduction with no row left adds nothing)
     const int n_units  = g.count && g.count_dim == 2 && g.count_base > 0 && K == 0 ? 0 : n_tiles * g.splits * g.batch;
     const int n_kb     = (K + kBK - 1) / kBK;
-    const int kb_slice = (n_kb + g.splits - 1) / g.splits;
+    const int kb_slice = ((n_kb + g.splits - 1) / g.splits + 1) & ~1;  // (whole chunks)
     const int first    = blockIdx.x / CG, step = gridDim.x / CG;
 
     auto decode = [&](int u, int &t_m, int &t_n, int &kb0, int &kb1, int &batch, int &split) {
-        int t = u % n_tiles;
-        u /= n_tiles;
-        split = u % g.splits;
-        batch = u / g.splits;
+        int t = u;
+        split = batch = 0;
+        if (u >= n_tiles)
+        {
+            u /= n_tiles;
+            t -= u * n_tiles;
+            batch = u;
+            if (g.splits > 1)
+            {
+                batch = u / g.splits;
+                split = u - batch * g.splits;
+            }
+        }
         kb0   = min(n_kb, split * kb_slice);
         kb1   = min(n_kb, kb0 + kb_slice);
         if (g.sym)
@@ -255,8 +277,8 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
             const int grp       = t / per_group;
             const int gsz       = min(tiles_m - grp * kGroupM, kGroupM);
             const int local     = t - grp * per_group;
-            t_m                 = grp * kGroupM + local % gsz;
             t_n                 = local / gsz;
+            t_m                 = grp * kGroupM + local - t_n * gsz;
         }
     };
 
@@ -280,7 +302,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                 for (int kb = kb0; kb < kb1; ++kb, ++gk)
                 {
                     const int s = gk % C::stages;
-                    if (!ptx::mbar_wait(&done_bar[s], ((gk / C::stages) & 1) ^ 1, abort_f))
+                    if (!ptx::mbar_wait(&empty_bar[s], ((gk / C::stages) & 1) ^ 1, abort_f))
                     {
                         ok = false;
                         break;
@@ -339,11 +361,21 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
             {
                 int t_m, t_n, kb0, kb1, batch, split;
                 decode(u, t_m, t_n, kb0, kb1, batch, split);
-                for (int kb = kb0; kb < kb1; ++kb, ++gk, ++gc)
+                int c = 0, chunk_end = kb0;
+                for (int kb = kb0; kb < kb1; ++kb, ++gk)
                 {
+                    const bool opens = kb == chunk_end;
+                    if (opens)
+                    {
+                        chunk_end = min(kb1, kb + chunk_blocks<SCALED>(c++));
+                        if (!ptx::mbar_wait(&acc_empty[gc & 1], ((gc >> 1) & 1) ^ 1, abort_f))
+                        {
+                            ok = false;
+                            break;
+                        }
+                    }
                     const int buf = gc & 1, s = gk % C::stages;
-                    if (!ptx::mbar_wait(&acc_empty[buf], ((gc >> 1) & 1) ^ 1, abort_f) ||
-                        !ptx::mbar_wait(&full_bar[s], (gk / C::stages) & 1, abort_f))
+                    if (!ptx::mbar_wait(&full_bar[s], (gk / C::stages) & 1, abort_f))
                     {
                         ok = false;
                         break;
@@ -365,17 +397,25 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
 #pragma unroll
                         for (int k = 0; k < kBK / 16; ++k)
                         {
-                            mma(sa + C::a_bytes + k * a_step, sb + k * b_step, k != 0);
+                            mma(sa + C::a_bytes + k * a_step, sb + k * b_step, !opens || k != 0);
                             mma(sa + k * a_step, sb + C::b_bytes + k * b_step, 1);
                         }
                     }
 #pragma unroll
                     for (int k = 0; k < kBK / 16; ++k)
-                        mma(sa + k * a_step, sb + k * b_step, TERMS == 3 || k != 0);
+                        mma(sa + k * a_step, sb + k * b_step, TERMS == 3 || !opens || k != 0);
                     if (CG == 2)
-                        ptx::mma_commit_pair_both(&done_bar[s]);
+                        ptx::mma_commit_pair_both(&empty_bar[s]);
                     else
-                        ptx::mma_commit(&done_bar[s]);
+                        ptx::mma_commit(&empty_bar[s]);
+                    if (kb + 1 == chunk_end)
+                    {
+                        if (CG == 2)
+                            ptx::mma_commit_pair_both(&acc_full[buf]);
+                        else
+                            ptx::mma_commit(&acc_full[buf]);
+                        ++gc;
+                    }
                 }
             }
         }
@@ -402,25 +442,25 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
 #pragma unroll
             for (int i = 0; i < C::strip; ++i)
                 acc[i] = 0.f;
-            // scales of this strip: rows of A through `row` blocks, columns of B in blocks of 64 (at most two)
-            auto scale_a = [&](int kb) -> float {
-                return g.a_mn ? g.sa[(kb >> 1) * g.lda_s + min(at.row >> 6, g.lda_s - 1)] : g.sa[(min(m0, M - 1) >> 7) * g.lda_s + kb];
-            };
-            auto scale_b = [&](int kb, int blk) -> float {
-                const int n = min(at.col + 64 * blk, g.N - 1);
-                return g.b_mn ? g.sb[(kb >> 1) * g.ldb_s + (n >> 6)] : g.sb[(n >> 7) * g.ldb_s + kb];
-            };
-            for (int kb = kb0; kb < kb1; ++kb, ++gc)
+            // scales: one of A's 128 rows, one of B's 128 columns (a strip crosses no block of 128)
+            const float *pa = nullptr, *pb = nullptr;
+            if (SCALED)
             {
-                const int buf = gc & 1, s = gc % C::stages;
-                float f0 = 1.f, f1 = 1.f;
+                const int m = min(m0, M - 1) >> 7, n = min(at.col, g.N - 1) >> 7;
+                pa          = g.sa ? g.sa + (g.a_mn ? m : m * g.lda_s) : nullptr;
+                pb          = g.sb ? g.sb + (g.b_mn ? n : n * g.ldb_s) : nullptr;
+            }
+            for (int kb = kb0, c = 0; kb < kb1; ++c, ++gc)
+            {
+                const int buf = gc & 1;
+                float f       = 1.f;
                 if (SCALED)
                 {
-                    const float a = g.sa ? scale_a(kb) : 1.f;
-                    f0            = a * (g.sb ? scale_b(kb, 0) : 1.f);
-                    f1            = C::strip > 64 ? a * (g.sb ? scale_b(kb, 1) : 1.f) : f0;
+                    const int k = kb >> 1;
+                    f           = (pa ? __ldg(pa + (g.a_mn ? k * g.lda_s : k)) : 1.f) * (pb ? __ldg(pb + (g.b_mn ? k * g.ldb_s : k)) : 1.f);
                 }
-                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&done_bar[s], (gc / C::stages) & 1, abort_f));
+                kb += chunk_blocks<SCALED>(c);
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[buf], (gc >> 1) & 1, abort_f));
                 if (!ok)
                     break;
                 ptx::tc_fence_after_sync();
@@ -433,7 +473,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        acc[32 * j + i] = SCALED ? fmaf(__uint_as_float(r[i]), j < 2 ? f0 : f1, acc[32 * j + i])
+                        acc[32 * j + i] = SCALED ? fmaf(__uint_as_float(r[i]), f, acc[32 * j + i])
                                                  : acc[32 * j + i] + __uint_as_float(r[i]);
                 }
                 ptx::tc_fence_before_sync();
@@ -523,8 +563,8 @@ int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::P
     int rc;
     if ((rc = make_tmap_split16(&tm.a, A, g.a_mn ? kBK : 128)) || (rc = make_tmap_split16(&tm.b, B, g.b_mn ? kBK : C::bn_cta)))
         return rc;
-    g.sa = A.scale, g.lda_s = A.cols_pad / 64;
-    g.sb = B.scale, g.ldb_s = B.cols_pad / 64;
+    g.sa = A.scale, g.lda_s = (A.cols_pad + 127) / 128;
+    g.sb = B.scale, g.ldb_s = (B.cols_pad + 127) / 128;
     static int resident = 0;  // CTAs (pairs) the GPU holds at once; one device per process
     if (resident == 0)
     {

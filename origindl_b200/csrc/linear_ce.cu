@@ -5,7 +5,7 @@
 //
 // Rows without a label are left out before anything is computed: the labels pass lists the n others, x is gathered through that
 // list while it is split into halves, and every kernel behind it reads n on the device (a batch that is half padding costs
-// half).  The matrices are split-fp16 (gemm_split16.cuh): W and x once, with a power of two per 128 x 64 tile.
+// half).  The matrices are split-fp16 (gemm_split16.cuh): W and x once, with a power of two per 128 x 128 tile.
 // Loss alone: the logits' GEMM keeps a running maximum and sum of each row's strip of 128 columns in the epilogue's registers
 // and writes those two numbers, nothing else.  With gradients: the rows are taken in pieces whose logits fit kPieceBytes; the
 // same epilogue also stores the logits, and once the row statistics are joined one pass turns them into P in place (the 4 bytes
@@ -517,7 +517,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     if (!grads && !g_lce_piece && linear_ce_few_eligible(M, N, K, w, w_layout))
         return linear_ce_few(x, w, b, labels, is64, ignore_index, M, N, K, w_layout, loss, lse_out, precision, stream);
     const bool out_in  = w_layout == ODL_W_OUT_IN;
-    const int kp = s16::pad64(K), np = s16::pad64(N);
+    const int kp = s16::pad64(K), np = s16::pad64(N), ks = (kp + 127) / 128;  // (scales of 128 columns)
     const int64_t m_pad = (M + 127) / 128 * 128;
 
     // rows per piece
@@ -540,7 +540,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     const int sum_rows    = (R + 127) / 128 * sm_cols < s16::sm_count() ? 32 : 128;
     const bool own_lse    = sum_rows == 32 && sm_cols == 1;  // (a block over all columns: nobody else needs its rows' lse)
 
-    const size_t scale_w = a256((N + 127) / 128 * (kp / 64) * 4), scale_x = a256(m_pad / 128 * (kp / 64) * 4);
+    const size_t scale_w = a256((N + 127) / 128 * ks * 4), scale_x = a256(m_pad / 128 * ks * 4);
     const size_t bytes   = 3 * a256(M * 4) + 256 + a256(N * static_cast<int64_t>(kp) * 4) + scale_w + a256(m_pad * kp * 4) + scale_x +
                          a256(static_cast<int64_t>(strips) * R * 8) + 3 * a256(piece * 4) + a256(M * 4) +
                          (grads ? a256(piece * np * 4) : 0) + (db ? a256(m_pad / sum_rows * static_cast<int64_t>(np) * 4) : 0) +
@@ -575,7 +575,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     {
         s16::ZeroRows zero{pos_of, dx, lse_out, (int)M, (int)K, 0};
         if (dx || lse_out)
-            zero.blocks = (int)((M + 7) / 8 < 592 ? (M + 7) / 8 : 592);
+            zero.blocks = (int)((M + 15) / 16 < 296 ? (M + 15) / 16 : 296);
         if ((rc = s16::split16_encode(s16::encode_job(w, out_in ? K : N, !out_in, (int)N, (int)K, nullptr, nullptr, W, w_scale),
                                       s16::encode_job(x, K, 0, (int)M, (int)K, idx, &cnt->count, X, x_scale), zero, stream)))
             return rc;
@@ -588,7 +588,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
         Split16 Xp = X;
         Xp.data += base * X.pitch;
         Xp.rows  = rows;
-        Xp.scale = x_scale + base / 128 * (kp / 64);
+        Xp.scale = x_scale + base / 128 * ks;
         GemmArgs g   = gz;
         g.M          = rows;
         g.count      = &cnt->count;

@@ -9,8 +9,9 @@
 // smallest: the grid 2^-39 of an entry adds at most 2^-39 sqrt(rows cols) to the Frobenius norm 1 of X, less than the 2^-24 of
 // fp32 itself up to 2^30 entries.  A and S are symmetric: their GEMMs compute the tiles on and above the diagonal and write each
 // twice, which leaves s s l + s^3 + 2 s s l operations a step (s, l the smaller and larger side) of the 2 + 2 + 2.
-// a X is folded into S (a on the diagonal), so a step is three GEMMs and nothing else; the last one's epilogue writes the result
-// or the updated parameters.
+// a X is folded into S (a on the diagonal), and b A into the square: with A' = A + h I, h = b / 2c, S = c A'^2 + (a - c h^2) I,
+// so that no epilogue reads a matrix.  A step is three GEMMs and nothing else; the last one's epilogue writes the result or the
+// updated parameters.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -216,54 +217,29 @@ __device__ __forceinline__ void store_split_mirror(__half *base, int64_t pitch, 
     }
 }
 
-// A = X X^T or S = a I + b A + c A^2 (poly): symmetric, halves, both triangles
-template <bool POLY>
+// A symmetric result in halves, both triangles: alpha * accumulator + diag on the diagonal
 struct EpiSym
 {
     struct Params
     {
         __half *out;
-        const __half *a;  // POLY: A
         int64_t pitch, stride;
         int cols_pad;
-        float alpha;      // accumulator -> value * scale of the halves
+        float alpha, diag;  // in units of the halves
     };
     template <int NC>
     static __device__ __forceinline__ void store(const Params &p, const GemmArgs &, const TileAt &at, float (&v)[NC], float *)
     {
-        const int64_t mat = at.batch * p.stride;
-        if (POLY)
-        {
-            const __half *row = p.a + mat + min(at.row, at.rows - 1) * p.pitch;
-            const float b     = at.row < at.rows ? kNsB * kSs / kSa : 0.f;  // (rows past the last mirror into padding: zeros)
 #pragma unroll
-            for (int i = 0; i < NC; i += 8)
-            {
-                const int c = min(at.col + i, p.cols_pad - 8);
-                const uint4 h = __ldg(reinterpret_cast<const uint4 *>(row + (c >> 6) * 128 + (c & 63)));
-                const uint4 l = __ldg(reinterpret_cast<const uint4 *>(row + (c >> 6) * 128 + (c & 63) + 64));
-                const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                {
-                    const float2 fh = __half22float2(*reinterpret_cast<const __half2 *>(&hw[j]));
-                    const float2 fl = __half22float2(*reinterpret_cast<const __half2 *>(&lw[j]));
-                    v[i + 2 * j]     = fmaf(v[i + 2 * j], p.alpha, (fh.x + fl.x) * b);
-                    v[i + 2 * j + 1] = fmaf(v[i + 2 * j + 1], p.alpha, (fh.y + fl.y) * b);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-                if (at.col + i == at.row && at.row < at.rows)
-                    v[i] += kNsA * kSs;
-        }
-        else
+        for (int i = 0; i < NC; ++i)
+            v[i] *= p.alpha;
+        if (at.tm == at.tn)
         {
 #pragma unroll
             for (int i = 0; i < NC; ++i)
-                v[i] *= p.alpha;
+                v[i] += at.col + i == at.row && at.row < at.rows ? p.diag : 0.f;
         }
-        __half *out = p.out + mat;
+        __half *out = p.out + at.batch * p.stride;
         if (at.row < at.rows)
             store_split_row<NC>(out + at.row * p.pitch, at.col, p.cols_pad, v);
         if (at.tm != at.tn)
@@ -441,9 +417,10 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
     for (int k = 0; k < steps; ++k)
     {
         const Split16 MX = matrix(x[k & 1], rows, xc, x_stride);
-        const EpiSym<false>::Params ea{A, nullptr, 2 * mc, m_stride, mc, kSa / (kSx * kSx)};
-        const EpiSym<true>::Params es{S, A, 2 * mc, m_stride, mc, kNsC * kSs / (kSa * kSa)};
-        if ((rc = gemm<EpiSym<false>>(plan_a, terms, MX, MX, ga, ea, stream)) || (rc = gemm<EpiSym<true>>(plan_s, terms, MA, MA, gs, es, stream)))
+        // A holds X X^T + h I, h = b / 2c: S = a I + b X X^T + c (X X^T)^2 = c A^2 + (a - c h^2) I
+        const EpiSym::Params ea{A, 2 * mc, m_stride, mc, kSa / (kSx * kSx), kNsH * kSa};
+        const EpiSym::Params es{S, 2 * mc, m_stride, mc, kNsC * kSs / (kSa * kSa), kNsD * kSs};
+        if ((rc = gemm<EpiSym>(plan_a, terms, MX, MX, ga, ea, stream)) || (rc = gemm<EpiSym>(plan_s, terms, MA, MA, gs, es, stream)))
             return rc;
         if (k + 1 < steps)
         {

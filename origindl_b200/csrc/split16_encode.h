@@ -9,7 +9,7 @@ namespace odl
 namespace s16
 {
 
-// out (rows x cols, tile scales in `scale`, [ceil(rows / 128)][cols_pad / 64]) = src, row-major with pitch ld, or its transpose
+// out (rows x cols, tile scales in `scale`, [ceil(rows / 128)][ceil(cols_pad / 128)]) = src, row-major with pitch ld, or its transpose
 // (element (r, c) at src[c * ld + r]).  gather (not with transposed): row r of out is row gather[r] of src, r < *count; the rows
 // behind, up to a multiple of 128, become zeros (out holds that many).
 struct EncodeJob
@@ -19,7 +19,7 @@ struct EncodeJob
     __half *out;
     float *scale;
     int64_t ld, pitch, blocks;
-    int transposed, rows, cols, blocks_c;
+    int transposed, rows, cols, cols_pad, blocks_c;
 };
 EncodeJob encode_job(const float *src, int64_t ld, int transposed, int rows, int cols, const int *gather, const int *count, const Split16 &out, float *scale);
 
