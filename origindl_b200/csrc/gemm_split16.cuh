@@ -11,11 +11,13 @@
 //
 // The kernel: persistent, one CTA (128 x BN tiles) or a CTA pair (256 x 256, tcgen05 cta_group::2) per SM (pair), warp 0 feeds a
 // ring of 64-deep K-blocks by TMA (no multicast), one thread of warp 1 issues the MMAs, eight warps drain the accumulator.
-// TMEM accumulation truncates (a step of the accumulator per instruction), so an accumulator holds 128 of the reduction only: two
-// TMEM buffers alternate, and the drain adds them up in fp32 registers, scaled by the tiles' s where the operands have many.  Of
-// each K-block the small products go first, so that only four instructions truncate at full size.  The epilogue holds up the
-// drain (8 to 18 thousand cycles a tile, when all SMs store at once, against 1536 a K-block); the MMA thread runs two buffers
-// ahead of it, and where no scales are in the way the first two buffers of a tile take 256 of the reduction each.
+// TMEM accumulation truncates (a step of the accumulator per instruction, always towards zero), so an accumulator holds little of
+// the reduction: two TMEM buffers alternate, and the drain adds them up in fp32 registers, scaled by the tiles' s where the
+// operands have many.  Of each K-block the small products go first, so that only four instructions truncate at full size.  A loss
+// takes chunks of 128, which its tile scales cover; Newton-Schulz, whose steps amplify errors, 64 (five steps of 300 x 900: 1.7e-6
+// off in the 2-norm, 3.7e-6 with 128; plain fp32 products 2.0e-6).  The epilogue holds up the drain (8 to 18 thousand cycles a
+// tile, when all SMs store at once, against 1536 a K-block) and the MMA thread runs only two chunks ahead of it: long
+// reductions without scales begin with two chunks of 128.
 // Every wait is bounded; a wait that gives up raises the abort flag, which releases the others, and the error flag.
 #pragma once
 #include <cuda.h>
@@ -66,13 +68,14 @@ struct GemmArgs
     const int *count;          // device: rows that exist from row 0 of the whole batch; nullptr = all
     int count_base, count_dim; // this call starts at count_base; 1: limits M, 2: limits K
     const float *sa, *sb;      // per-tile scales or nullptr
+    int diag;                  // where B's 128 x 128 blocks on the diagonal differ: they come from the third map, [rows][128]
     int lda_s, ldb_s;
     int *err;
 };
 
 struct Tmaps
 {
-    CUtensorMap a, b;
+    CUtensorMap a, b, d;
 };
 
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
@@ -146,11 +149,11 @@ struct Cfg
     static constexpr int strip   = BN / 2;  // columns of the tile one epilogue warp holds
 };
 
-// K-blocks of a tile's c-th chunk (what one accumulator buffer holds); 128 of the reduction is also what a tile scale covers
+// K-blocks of a tile's c-th chunk (what one accumulator buffer holds) of n
 template <bool SCALED>
-__device__ __forceinline__ int chunk_blocks(int c)
+__device__ __forceinline__ int chunk_blocks(int c, int n)
 {
-    return SCALED || c >= 2 ? 2 : 4;
+    return SCALED || (c < 2 && n >= 16) ? 2 : 1;
 }
 
 // what the epilogue is told about a tile
@@ -328,7 +331,9 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                             for (int j = 0; j < 2; ++j)
                                 load(sa + j * 8192, &tm.a, 2 * m0 + 128 * j + 64 * p, kb * kBK);
                         uint8_t *sb = st + C::parts * C::a_bytes + p * C::b_bytes;
-                        if (!g.b_mn)
+                        if (g.diag && (kb >> 1) == (b0 >> 7))
+                            load(sb, &tm.d, 128 * (kb & 1) + 64 * p, b0);
+                        else if (!g.b_mn)
                             load(sb, &tm.b, 128 * kb + 64 * p, b0);
                         else
                             for (int j = 0; j < C::bn_cta / 64; ++j)
@@ -367,7 +372,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                     const bool opens = kb == chunk_end;
                     if (opens)
                     {
-                        chunk_end = min(kb1, kb + chunk_blocks<SCALED>(c++));
+                        chunk_end = min(kb1, kb + chunk_blocks<SCALED>(c++, kb1 - kb0));
                         if (!ptx::mbar_wait(&acc_empty[gc & 1], ((gc >> 1) & 1) ^ 1, abort_f))
                         {
                             ok = false;
@@ -459,7 +464,7 @@ gemm_split16_kernel(const __grid_constant__ Tmaps tm, const GemmArgs g, const ty
                     const int k = kb >> 1;
                     f           = (pa ? __ldg(pa + (g.a_mn ? k * g.lda_s : k)) : 1.f) * (pb ? __ldg(pb + (g.b_mn ? k * g.ldb_s : k)) : 1.f);
                 }
-                kb += chunk_blocks<SCALED>(c);
+                kb += chunk_blocks<SCALED>(c, kb1 - kb0);
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&acc_full[buf], (gc >> 1) & 1, abort_f));
                 if (!ok)
                     break;
@@ -555,13 +560,17 @@ int launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaS
 }
 
 template <int CG, int BN, int TERMS, bool SCALED, class Epi>
-int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::Params &ep, cudaStream_t stream)
+int launch(const Split16 &A, const Split16 &B, GemmArgs g, const typename Epi::Params &ep, cudaStream_t stream, const Split16 *D)
 {
     using C     = Cfg<CG, BN, TERMS>;
     auto kernel = gemm_split16_kernel<CG, BN, TERMS, SCALED, Epi>;
     Tmaps tm;
     int rc;
     if ((rc = make_tmap_split16(&tm.a, A, g.a_mn ? kBK : 128)) || (rc = make_tmap_split16(&tm.b, B, g.b_mn ? kBK : C::bn_cta)))
+        return rc;
+    tm.d   = tm.b;
+    g.diag = D != nullptr;
+    if (D && (rc = make_tmap_split16(&tm.d, *D, C::bn_cta)))
         return rc;
     g.sa = A.scale, g.lda_s = (A.cols_pad + 127) / 128;
     g.sb = B.scale, g.ldb_s = (B.cols_pad + 127) / 128;
@@ -613,13 +622,14 @@ struct Plan
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, int terms, int batch, bool may_split, bool sym = false);
 
 template <int TERMS, bool SCALED, class Epi>
-int launch_plan(const Plan &plan, const Split16 &A, const Split16 &B, const GemmArgs &g, const typename Epi::Params &ep, cudaStream_t stream)
+int launch_plan(const Plan &plan, const Split16 &A, const Split16 &B, const GemmArgs &g, const typename Epi::Params &ep, cudaStream_t stream,
+                const Split16 *D = nullptr)
 {
     if (plan.cg == 2)
-        return launch<2, 256, TERMS, SCALED, Epi>(A, B, g, ep, stream);
+        return launch<2, 256, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
     if (plan.bn == 128)
-        return launch<1, 128, TERMS, SCALED, Epi>(A, B, g, ep, stream);
-    return launch<1, 64, TERMS, SCALED, Epi>(A, B, g, ep, stream);
+        return launch<1, 128, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
+    return launch<1, 64, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
 }
 
 }  // namespace s16

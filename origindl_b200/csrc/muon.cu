@@ -9,9 +9,10 @@
 // smallest: the grid 2^-39 of an entry adds at most 2^-39 sqrt(rows cols) to the Frobenius norm 1 of X, less than the 2^-24 of
 // fp32 itself up to 2^30 entries.  A and S are symmetric: their GEMMs compute the tiles on and above the diagonal and write each
 // twice, which leaves s s l + s^3 + 2 s s l operations a step (s, l the smaller and larger side) of the 2 + 2 + 2.
-// a X is folded into S (a on the diagonal), and b A into the square: with A' = A + h I, h = b / 2c, S = c A'^2 + (a - c h^2) I,
-// so that no epilogue reads a matrix.  A step is three GEMMs and nothing else; the last one's epilogue writes the result or the
-// updated parameters.
+// a X is folded into S (a on the diagonal), and b A into the product: S = a I + c A (A + h I), h = b / c, so that no epilogue reads
+// a matrix.  A + h I differs from A in the blocks on the diagonal alone, and only those are kept a second time.  (The square
+// completed, c (A + h/2 I)^2 + d I, would need one operand, but its terms of order 1 cancel: 1.5 times the error.)  A step is
+// three GEMMs and nothing else; the last one's epilogue writes the result or the updated parameters.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -217,7 +218,8 @@ __device__ __forceinline__ void store_split_mirror(__half *base, int64_t pitch, 
     }
 }
 
-// A symmetric result in halves, both triangles: alpha * accumulator + diag on the diagonal
+// A symmetric result in halves, both triangles: alpha * accumulator (+ diag on the diagonal); with `blocks` its 128 x 128 blocks on
+// the diagonal, `blocks_diag` added on the diagonal, a second time
 struct EpiSym
 {
     struct Params
@@ -226,6 +228,9 @@ struct EpiSym
         int64_t pitch, stride;
         int cols_pad;
         float alpha, diag;  // in units of the halves
+        __half *blocks;     // [row][128 columns], blocks_stride halves from matrix to matrix
+        int64_t blocks_stride;
+        float blocks_diag;
     };
     template <int NC>
     static __device__ __forceinline__ void store(const Params &p, const GemmArgs &, const TileAt &at, float (&v)[NC], float *)
@@ -242,6 +247,14 @@ struct EpiSym
         __half *out = p.out + at.batch * p.stride;
         if (at.row < at.rows)
             store_split_row<NC>(out + at.row * p.pitch, at.col, p.cols_pad, v);
+        if (p.blocks && at.row >> 7 == at.col >> 7)  // (the same for a warp)
+        {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                v[i] += at.col + i == at.row && at.row < at.rows ? p.blocks_diag : 0.f;
+            if (at.row < at.rows)
+                store_split_row<NC>(p.blocks + at.batch * p.blocks_stride + at.row * 256, at.col & 127, 128, v);
+        }
         if (at.tm != at.tn)
             store_split_mirror<NC>(out, p.pitch, at.row - at.lane, at.col, at.rows, p.cols_pad, at.lane, v);
     }
@@ -352,9 +365,10 @@ __global__ void __launch_bounds__(256) muon_direct_kernel(const __half *__restri
 }
 
 template <class Epi>
-int gemm(const s16::Plan &plan, int terms, const Split16 &A, const Split16 &B, const GemmArgs &g, const typename Epi::Params &ep, cudaStream_t stream)
+int gemm(const s16::Plan &plan, int terms, const Split16 &A, const Split16 &B, const GemmArgs &g, const typename Epi::Params &ep, cudaStream_t stream,
+         const Split16 *D = nullptr)
 {
-    return terms == 3 ? s16::launch_plan<3, false, Epi>(plan, A, B, g, ep, stream) : s16::launch_plan<1, false, Epi>(plan, A, B, g, ep, stream);
+    return terms == 3 ? s16::launch_plan<3, false, Epi>(plan, A, B, g, ep, stream, D) : s16::launch_plan<1, false, Epi>(plan, A, B, g, ep, stream, D);
 }
 
 int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, EpiOut::Params out, int64_t batch, int64_t rows, int64_t cols,
@@ -371,15 +385,16 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
     }
     const int xc = s16::pad64(cols), mc = s16::pad64(m);
     // 256-byte multiples: rows are whole blocks of 64 columns
-    const int64_t x_stride = rows * 2 * xc, m_stride = m * 2 * mc;
+    const int64_t x_stride = rows * 2 * xc, m_stride = m * 2 * mc, d_stride = m * 2 * 128;
     int64_t blocks         = (n / 4 + 1023) / 1024;
     blocks                 = blocks < 1 ? 1 : blocks > kNormBlocks ? kNormBlocks : blocks;
-    int rc = arena_begin(2 * a256(batch * x_stride * 2) + 2 * a256(batch * m_stride * 2) + a256(batch * blocks * 8), stream);
+    int rc = arena_begin(2 * a256(batch * x_stride * 2) + 2 * a256(batch * m_stride * 2) + a256(batch * d_stride * 2) + a256(batch * blocks * 8), stream);
     if (rc)
         return rc;
     __half *x[2]    = {static_cast<__half *>(arena_alloc(batch * x_stride * 2)), static_cast<__half *>(arena_alloc(batch * x_stride * 2))};
     __half *A       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
     __half *S       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
+    __half *D       = static_cast<__half *>(arena_alloc(batch * d_stride * 2));  // the blocks of A + h I on the diagonal
     double *partial = static_cast<double *>(arena_alloc(batch * blocks * 8));
     auto al16       = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
     const bool vec  = !(n & 3) && al16(g) && al16(buf) && al16(p);
@@ -413,14 +428,13 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
         s.data = d, s.pitch = 2 * c_pad, s.rows = (int)r, s.cols_pad = c_pad, s.batch = (int)batch, s.batch_stride = stride;
         return s;
     };
-    const Split16 MA = matrix(A, m, mc, m_stride), MS = matrix(S, m, mc, m_stride);
+    const Split16 MA = matrix(A, m, mc, m_stride), MS = matrix(S, m, mc, m_stride), MD = matrix(D, m, 128, d_stride);
     for (int k = 0; k < steps; ++k)
     {
         const Split16 MX = matrix(x[k & 1], rows, xc, x_stride);
-        // A holds X X^T + h I, h = b / 2c: S = a I + b X X^T + c (X X^T)^2 = c A^2 + (a - c h^2) I
-        const EpiSym::Params ea{A, 2 * mc, m_stride, mc, kSa / (kSx * kSx), kNsH * kSa};
-        const EpiSym::Params es{S, 2 * mc, m_stride, mc, kNsC * kSs / (kSa * kSa), kNsD * kSs};
-        if ((rc = gemm<EpiSym>(plan_a, terms, MX, MX, ga, ea, stream)) || (rc = gemm<EpiSym>(plan_s, terms, MA, MA, gs, es, stream)))
+        const EpiSym::Params ea{A, 2 * mc, m_stride, mc, kSa / (kSx * kSx), 0.f, D, d_stride, kNsH * kSa};
+        const EpiSym::Params es{S, 2 * mc, m_stride, mc, kNsC * kSs / (kSa * kSa), kNsA * kSs, nullptr, 0, 0.f};
+        if ((rc = gemm<EpiSym>(plan_a, terms, MX, MX, ga, ea, stream)) || (rc = gemm<EpiSym>(plan_s, terms, MA, MA, gs, es, stream, &MD)))
             return rc;
         if (k + 1 < steps)
         {

@@ -10,8 +10,8 @@ namespace odl
 {
 
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-// a + b s + c s^2 = c (s + h)^2 + d
-constexpr float kNsH = static_cast<float>(-4.7750 / (2 * 2.0315)), kNsD = static_cast<float>(3.4445 - 4.7750 * 4.7750 / (4 * 2.0315));
+// b s + c s^2 = c s (s + h)
+constexpr float kNsH = static_cast<float>(-4.7750 / 2.0315);
 constexpr float kSx = 16384.f, kSa = 16384.f, kSs = 8192.f;  // halves hold value * this
 
 struct MomentumArgs
