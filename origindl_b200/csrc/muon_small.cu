@@ -3,7 +3,7 @@
 // A matrix belongs to a cluster of 1 to 8 CTAs.  X (taken with its short side as rows) lies in their shared memory for the whole
 // iteration, split-fp16 (gemm_split16.cuh, muon.cu), each CTA holding a range of columns; nothing but the gradient, the momentum
 // and the result touches global memory.  A step in each CTA:
-//   partial A = X_loc X_loc^T      (X_loc read K-major twice; up to four accumulators, so that each sums at most two blocks of 64)
+//   partial A = X_loc X_loc^T      (X_loc read K-major twice; as many accumulators as TMEM holds, so that each sums few blocks of 64)
 //   A = sum over the cluster       (each CTA adds a slice of columns of all partials in rank order, and writes its halves to all)
 //   S = a I + b A + c A^2          (every CTA the whole of it: 24 MMAs, less than moving it)
 //   X_loc = S X_loc                (the same X_loc read MN-major)
@@ -46,27 +46,27 @@ struct SmallArgs
     float eps;
 };
 
-// RB: rows of a block in shared memory (64 or 128); the MMAs' M is 128 either way, rows past RB are whatever follows (their
+// RB: rows of a block in shared memory (16, 32, 64 or 128); the MMAs' M is 128 whatever RB, rows past RB are whatever follows (their
 // accumulator lanes are not read).  A, S and the partial A in fp32 take turns in one place: the partial sums are read before A is
 // written, and every thread writes the elements of S over the ones of A that it has just read.
 template <int RB>
 struct SmallCfg
 {
-    static constexpr int block   = RB * 128;            // bytes of 64 columns of halves
-    static constexpr int max_blk = RB == 64 ? 8 : 5;    // (TMEM holds 512 columns of X; 224 KB)
-    static constexpr int sq      = RB / 64 * block;     // bytes of an RB x RB matrix of halves
+    static constexpr int block = RB * 128;                           // bytes of 64 columns of halves
+    static constexpr int sq    = RB > 64 ? 2 * block : block;        // bytes of an RB x RB matrix of halves
+    static constexpr int accs  = 512 / RB;                           // accumulators of partial A in TMEM
     // X: hi blocks, lo blocks; A / S: hi, lo; the cluster's reduced slices of A (fp32)
     __host__ __device__ static constexpr int x_lo(int blocks) { return blocks * block; }
     __host__ __device__ static constexpr int a_hi(int blocks) { return 2 * blocks * block; }
     __host__ __device__ static constexpr int red(int blocks) { return a_hi(blocks) + 2 * sq; }
-    // (an M = 128 read from the last RB = 64 block ends a block further on)
+    // (an M = 128 read of the last matrix ends 128 rows from its start)
     __host__ __device__ static constexpr int aux(int blocks, int cluster)
     {
-        const int r = cluster > 1 ? 2 * sq / cluster : 0;
-        return red(blocks) + (RB == 64 && r < block ? block : r);
+        const int r = cluster > 1 ? RB * RB * 4 / cluster : 0, past = (128 - RB) * 128;
+        return red(blocks) + (r > past ? r : past);
     }
     __host__ __device__ static constexpr int bytes(int blocks, int cluster) { return 1024 + aux(blocks, cluster) + 512; }
-    __host__ __device__ static constexpr bool fits(int blocks, int cluster) { return blocks <= max_blk && bytes(blocks, cluster) <= 227 * 1024; }
+    __host__ __device__ static constexpr bool fits(int blocks, int cluster) { return bytes(blocks, cluster) <= 227 * 1024; }
 };
 
 // byte of element (row, col) inside a matrix of 64-column blocks, 128-byte swizzle
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
             for (int b = 0; b < p.blocks; ++b)
 #pragma unroll 1
                 for (int i = warp; i < RB; i += 64)
-                    body(std::integral_constant<bool, false>(), std::integral_constant<int, 8>(), i, 64 * b + 2 * lane);
+                    body(std::integral_constant<bool, false>(), std::integral_constant<int, (RB < 64 ? RB / 8 : 8)>(), i, 64 * b + 2 * lane);
         }
         else
         {
@@ -326,31 +326,35 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
             for (int b = 0; b < p.blocks; ++b)
             {
                 const uint64_t hi = k_major(b * C::block), lo = k_major(o_xlo + b * C::block);
-                products(tmem + (b & 3) * 128, hi, lo, hi, lo, 4, along_row, along_row, idesc, b >= 4);
+                products(tmem + b % C::accs * RB, hi, lo, hi, lo, 4, along_row, along_row, idesc, b >= C::accs);
             }
             ptx::mma_commit(bar);
         }
         finish_mmas();
-        const int accs    = p.blocks < 4 ? p.blocks : 4;
-        constexpr float f = kSa / (kSx * kSx), f_out = 1.f / (kSs * kSx);
+        const int accs    = p.blocks < C::accs ? p.blocks : C::accs;
+        constexpr float f = kSa / (kSx * kSx);
         if (mine)
         {
-            float *part = reinterpret_cast<float *>(sm + o_ahi);
-            for (int c = c_from; c < c_to; c += 32)
+            float *part     = reinterpret_cast<float *>(sm + o_ahi);
+            constexpr int W = RB < 64 ? 8 : 32;  // columns at a time: accumulators lie RB columns apart
+            for (int c = c_from; c < c_to; c += W)
             {
-                float v[32];
+                float v[W];
                 for (int a = 0; a < accs; ++a)
                 {
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32(lanes + a * 128 + c, r);  // (columns past c_to are other sums or unused: not written)
+                    uint32_t r[W];
+                    if constexpr (W == 8)
+                        s16::tmem_ld_32x8(lanes + a * RB + c, r);
+                    else
+                        ptx::tmem_ld_32x32(lanes + a * RB + c, r);
                     ptx::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < W; ++i)
                         v[i] = a ? v[i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    if (c + i < c_to)
+                for (int i = 0; i < W; i += 8)
+                    if (c + i < c_to && row < RB)
                     {
                         if (p.cluster == 1)
                         {
@@ -393,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
             }
             ptx::cluster_sync();
             // a thread: four rows of two columns; eight row groups and four column pairs a warp (shared-memory banks)
-            const int groups = RB / 32, n = p.s_pad / 8 * groups;
+            const int groups = (RB + 31) / 32, n = p.s_pad / 8 * groups;
+            const bool in    = 4 * (lane & 7) < RB;  // (RB = 16: half the lanes)
             for (int k0 = warp; k0 < n; k0 += 4 * (kThreads / 32))
             {
                 float4 v[4][2];
@@ -401,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
                 for (int t = 0; t < 4; ++t)
                 {
                     const int k = k0 + t * (kThreads / 32);
-                    const int j = k < n ? k / groups * 8 + 2 * (lane >> 3) : 0, i = k < n ? (k % groups) * 32 + 4 * (lane & 7) : 0;
+                    const int j = k < n ? k / groups * 8 + 2 * (lane >> 3) : 0, i = k < n && in ? (k % groups) * 32 + 4 * (lane & 7) : 0;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                     {
@@ -413,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
                 for (int t = 0; t < 4; ++t)
                 {
                     const int k = k0 + t * (kThreads / 32);
-                    if (k >= n)
+                    if (k >= n || !in)
                         break;
                     const int j = k / groups * 8 + 2 * (lane >> 3), i = (k % groups) * 32 + 4 * (lane & 7);
                     const float a0[4] = {v[t][0].x, v[t][0].y, v[t][0].z, v[t][0].w}, a1[4] = {v[t][1].x, v[t][1].y, v[t][1].z, v[t][1].w};
@@ -448,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
 #pragma unroll
                 for (int o = 0; o < 32; o += 8)
                 {
-                    if (c + o >= c_to)
+                    if (c + o >= c_to || row >= RB)
                         break;
                     const uint32_t at = place<RB>(row, c + o);  // (8 columns of a row lie together)
                     const uint4 ah = *reinterpret_cast<const uint4 *>(sm + o_ahi + at), al = *reinterpret_cast<const uint4 *>(sm + o_alo + at);
@@ -470,54 +475,46 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
             }
         threads_meet();
 
-        // X_loc = S X_loc
-        if (tid == 0)
+        // X_loc = S X_loc, 512 columns (TMEM) at a time
+        for (int n0 = 0; n0 < n_loc; n0 += 512)
         {
-            for (int n = 0; n < n_loc; n += 256)
+            const int width = n_loc - n0 < 512 ? n_loc - n0 : 512;
+            if (tid == 0)
             {
-                const int cols = n_loc - n < 256 ? n_loc - n : 256, at = n / 64 * C::block;
-                products(tmem + n, k_major(o_ahi), k_major(o_alo), rows_of_x(at), rows_of_x(o_xlo + at), ksq, along_row, along_rows,
-                         s16::idesc_f16(128, cols, false, true), 0);
-            }
-            ptx::mma_commit(bar);
-        }
-        finish_mmas();
-        if (mine)
-        {
-            const bool last = step + 1 == p.steps;
-            for (int c = h * (n_loc / 2); c < (h + 1) * (n_loc / 2); c += 32)
-            {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32(lanes + c, r);
-                ptx::tmem_ld_wait();
-                if (!last)
+                for (int n = 0; n < width; n += 256)
                 {
-#pragma unroll
-                    for (int o = 0; o < 32; o += 8)
+                    const int cols = width - n < 256 ? width - n : 256, at = (n0 + n) / 64 * C::block;
+                    products(tmem + n, k_major(o_ahi), k_major(o_alo), rows_of_x(at), rows_of_x(o_xlo + at), ksq, along_row, along_rows,
+                             s16::idesc_f16(128, cols, false, true), 0);
+                }
+                ptx::mma_commit(bar);
+            }
+            finish_mmas();
+            if (mine)
+                for (int c = h * (width / 2); c < (h + 1) * (width / 2); c += 32)
+                {
+                    uint32_t r[32];
+                    ptx::tmem_ld_32x32(lanes + c, r);
+                    ptx::tmem_ld_wait();
+                    if (row < RB)
                     {
-                        uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s16::split2(__uint_as_float(r[o + 2 * i]) * (1.f / kSs), __uint_as_float(r[o + 2 * i + 1]) * (1.f / kSs), hi[i], lo[i]);
-                        const uint32_t at                             = place<RB>(row, c + o);
-                        *reinterpret_cast<uint4 *>(sm + at)         = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(sm + o_xlo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        for (int o = 0; o < 32; o += 8)
+                        {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                s16::split2(__uint_as_float(r[o + 2 * i]) * (1.f / kSs), __uint_as_float(r[o + 2 * i + 1]) * (1.f / kSs), hi[i], lo[i]);
+                            const uint32_t at                             = place<RB>(row, n0 + c + o);
+                            *reinterpret_cast<uint4 *>(sm + at)         = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4 *>(sm + o_xlo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
                     }
                 }
-                else
-                {
-                    // the result in fp32, 256 bytes a row of a block, over X (dead); 16-byte pieces change places by the row
-                    float4 *to = reinterpret_cast<float4 *>(sm + ((c >> 6) * RB + row) * 256);
-#pragma unroll
-                    for (int o = 0; o < 32; o += 4)
-                        to[(((c & 32) + o) >> 2) ^ (row & 15)] = make_float4(__uint_as_float(r[o]) * f_out, __uint_as_float(r[o + 1]) * f_out,
-                                                                           __uint_as_float(r[o + 2]) * f_out, __uint_as_float(r[o + 3]) * f_out);
-                }
-            }
+            threads_meet();
         }
-        threads_meet();
     }
-    // ---- the result, by the threads and in the order that read the gradient --------------------------------------------------------
+    // ---- the result out of its halves (2^-23 of a value), by the threads and in the order that read the gradient --------------------
     float *const O = p.out.out + off, *const L = p.out.small ? p.out.small + off : nullptr;
     const bool two_out = !tall && !(p.cols & 1) && even(O) && even(L);
     batches([&](auto is_tall, auto n, int i, int c) {
@@ -534,8 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
         for (int t = 0; t < N; ++t)
         {
             const Pair q   = pair(is_tall, t, i, c);
-            const float2 x = *reinterpret_cast<const float2 *>(sm + ((q.c >> 6) * RB + q.i) * 256 + ((((q.c & 63) >> 2) ^ (q.i & 15)) << 4) + (q.c & 2) * 4);
-            const float o0 = ns_result(p.out, x.x, was[t][0]), o1 = ns_result(p.out, x.y, was[t][1]);
+            const uint32_t at = place<RB>(q.i, q.c);
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(sm + at)), lo = __half22float2(*reinterpret_cast<const __half2 *>(sm + o_xlo + at));
+            const float o0 = ns_result(p.out, (hi.x + lo.x) * (1.f / kSx), was[t][0]), o1 = ns_result(p.out, (hi.y + lo.y) * (1.f / kSx), was[t][1]);
             store_pair(O, q, two_out, o0, o1);
             if (L)
                 store_pair(L, q, two_out, tf32_small(o0), tf32_small(o1));
@@ -565,15 +563,50 @@ int cluster_for(int blocks, int64_t batch)
         c *= 2;
     return c;
 }
+int cluster_of(int s, int blocks, int64_t batch)
+{
+    return s <= 16 ? cluster_for<16>(blocks, batch) : s <= 32 ? cluster_for<32>(blocks, batch) : s <= 64 ? cluster_for<64>(blocks, batch) : cluster_for<128>(blocks, batch);
+}
+template <int RB>
+int launch_small(SmallArgs &k, int64_t batch, cudaStream_t stream)
+{
+    static bool set = false;
+    if (!set)
+    {
+        ODL_CUDA_TRY(cudaFuncSetAttribute(muon_small_kernel<RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        set = true;
+    }
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim          = dim3(static_cast<unsigned>(batch * k.cluster));
+    cfg.blockDim         = dim3(kThreads);
+    cfg.dynamicSmemBytes = SmallCfg<RB>::bytes(k.blocks, k.cluster);
+    cfg.stream           = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id               = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = k.cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs                = attr;
+    cfg.numAttrs             = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, muon_small_kernel<RB>, k);
+    ++g_launch_count;
+    if (e != cudaSuccess)
+    {
+        set_last_error("muon_small_kernel launch failed: %s", cudaGetErrorString(e));
+        return kCudaError;
+    }
+    return kOk;
+}
 }  // namespace
 
 bool muon_small_eligible(int64_t rows, int64_t cols, int steps)
 {
     const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
-    if (steps <= 0 || s > 128 || l > 64 * SmallCfg<64>::max_blk * kMaxCluster)
+    if (steps <= 0 || s > 128 || l > 1 << 20)
         return false;
     const int blocks = static_cast<int>((l + 63) / 64);
-    return (s <= 64 ? cluster_for<64>(blocks, 1 << 20) : cluster_for<128>(blocks, 1 << 20)) > 0;
+    return cluster_of(static_cast<int>(s), blocks, 1 << 20) > 0;
 }
 
 int muon_small(const float *p, float *g, float *buf, const MomentumArgs &a, const NsOut &out, int64_t batch, int64_t rows, int64_t cols, int steps,
@@ -585,40 +618,11 @@ int muon_small(const float *p, float *g, float *buf, const MomentumArgs &a, cons
     k.s = (int)(rows < cols ? rows : cols), k.l = (int)(rows < cols ? cols : rows);
     k.s_pad = (k.s + 15) / 16 * 16;
     k.steps = steps, k.terms = terms, k.eps = eps;
-    const bool narrow = k.s <= 64;
-    const int all     = (k.l + 63) / 64;
-    const int c       = narrow ? cluster_for<64>(all, batch) : cluster_for<128>(all, batch);
-    k.cluster = c;
-    k.blocks  = (all + c - 1) / c;
-    auto kernel    = narrow ? muon_small_kernel<64> : muon_small_kernel<128>;
-    const int smem = narrow ? SmallCfg<64>::bytes(k.blocks, c) : SmallCfg<128>::bytes(k.blocks, c);
-    static bool set[2] = {false, false};
-    if (!set[narrow])
-    {
-        ODL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-        set[narrow] = true;
-    }
-    cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim          = dim3(static_cast<unsigned>(batch * c));
-    cfg.blockDim         = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream           = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = c;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs                = attr;
-    cfg.numAttrs             = 1;
-    cudaError_t e            = cudaLaunchKernelEx(&cfg, kernel, k);
-    ++g_launch_count;
-    if (e != cudaSuccess)
-    {
-        set_last_error("muon_small_kernel launch failed: %s", cudaGetErrorString(e));
-        return kCudaError;
-    }
-    return kOk;
+    const int all = (k.l + 63) / 64;
+    k.cluster     = cluster_of(k.s, all, batch);
+    k.blocks      = (all + k.cluster - 1) / k.cluster;
+    return k.s <= 16 ? launch_small<16>(k, batch, stream) : k.s <= 32 ? launch_small<32>(k, batch, stream)
+         : k.s <= 64 ? launch_small<64>(k, batch, stream) : launch_small<128>(k, batch, stream);
 }
 
 }  // namespace odl

@@ -63,7 +63,7 @@ def bound(g, steps, precision):
     return want, 4 * far
 
 
-SHAPES = [(16, 700), (700, 16), (64, 4096), (64, 4097), (4000, 60), (128, 1536), (128, 1537), (1500, 120), (65, 1000), (100, 2000), (8, 64), (1, 1), (1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (63, 200), (128, 128), (129, 127), (100, 784), (784, 100),
+SHAPES = [(5, 5888), (16, 8192), (8192, 13), (17, 5120), (32, 8000), (6144, 40), (64, 6200), (2000, 31), (120, 1700), (16, 700), (700, 16), (64, 4096), (64, 4097), (4000, 60), (128, 1536), (128, 1537), (1500, 120), (65, 1000), (100, 2000), (8, 64), (1, 1), (1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (63, 200), (128, 128), (129, 127), (100, 784), (784, 100),
           (256, 256), (257, 300), (300, 257), (513, 1000), (1000, 513), (1024, 384), (1100, 1100), (260, 2000)]
 
 
