@@ -627,9 +627,10 @@ int launch_plan(const Plan &plan, const Split16 &A, const Split16 &B, const Gemm
 {
     if (plan.cg == 2)
         return launch<2, 256, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
-    if (plan.bn == 128)
-        return launch<1, 128, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
-    return launch<1, 64, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
+    if constexpr (!Epi::kSquare)  // (a symmetric output has square tiles)
+        if (plan.bn == 64)
+            return launch<1, 64, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
+    return launch<1, 128, TERMS, SCALED, Epi>(A, B, g, ep, stream, D);
 }
 
 }  // namespace s16

@@ -22,6 +22,12 @@ void *arena_alloc(size_t bytes);
 int check_device();  // the current device is the one odl_init bound
 int arena_begin(size_t bytes, cudaStream_t stream);
 int arena_end(cudaStream_t stream);
+// arena_end when a call that holds the arena returns, by whichever way
+struct ArenaUse
+{
+    cudaStream_t stream;
+    ~ArenaUse() { arena_end(stream); }
+};
 // Counts replacements of library-owned scratch blocks (arena, column-sum scratch): recorded graphs compare it.
 long long scratch_generation();
 void bump_scratch_generation();

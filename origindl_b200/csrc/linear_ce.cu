@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(1024) lce_labels_kernel(const void *__restrict
 // ---- epilogue of the logits' GEMM: row statistics of a strip of columns, the label's logit, the logits themselves --------
 struct EpiLogits
 {
+    static constexpr bool kSquare = false;
     struct Params
     {
         const float *bias;
@@ -210,6 +211,7 @@ struct EpiLogits
 // ---- epilogue of the gradients' GEMMs: scaled fp32 rows, through a row list, added to what is there, or as a slice -------
 struct EpiGrad
 {
+    static constexpr bool kSquare = false;
     struct Params
     {
         float *out;
@@ -548,6 +550,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     int rc = arena_begin(bytes, stream);
     if (rc)
         return rc;
+    const ArenaUse use{stream};
     auto take          = [&](size_t n) { return arena_alloc(n); };
     int *idx           = static_cast<int *>(take(M * 4));
     int *cls           = static_cast<int *>(take(M * 4));
@@ -641,7 +644,7 @@ int linear_cross_entropy(const float *x, const float *w, const float *b, const v
     if ((rc = s16::launch_after(lce_finish_kernel, dim3(1 + (db ? ((int)N + 255) / 256 : 0)), dim3(256), 0, stream, row_loss, colsum, np, sum_rows, (int)N,
                                 cnt, grad_scale, db, loss, device_error_flag())))
         return rc;
-    return arena_end(stream);
+    return kOk;
 }
 
 }  // namespace odl

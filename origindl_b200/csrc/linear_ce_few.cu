@@ -832,6 +832,7 @@ int linear_ce_few(const float *x, const float *w, const float *b, const void *la
     int rc = arena_begin(2 * xb + a256(static_cast<size_t>(rows) * parts * 8) + 5 * 512, stream);
     if (rc)
         return rc;
+    const ArenaUse use{stream};
     float *big      = static_cast<float *>(arena_alloc(xb));
     float *small    = static_cast<float *>(arena_alloc(xb));
     float2 *part    = static_cast<float2 *>(arena_alloc(static_cast<size_t>(rows) * parts * 8));
@@ -856,7 +857,7 @@ int linear_ce_few(const float *x, const float *w, const float *b, const void *la
         few_finish_kernel<<<(int)M, 256, 0, stream>>>(part, parts, idx, picked, words, row_loss, lse_out, loss, device_error_flag());
         ++g_launch_count;
         ODL_CUDA_TRY(cudaGetLastError());
-        return arena_end(stream);
+        return kOk;
     }
     FewTmaps tm;
     std::memset(&tm, 0, sizeof(tm));
@@ -874,7 +875,7 @@ int linear_ce_few(const float *x, const float *w, const float *b, const void *la
     few_finish_kernel<<<(int)M, 256, 0, stream>>>(part, parts, idx, picked, words, row_loss, lse_out, loss, device_error_flag());
     ++g_launch_count;
     ODL_CUDA_TRY(cudaGetLastError());
-    return arena_end(stream);
+    return kOk;
 }
 
 }  // namespace odl

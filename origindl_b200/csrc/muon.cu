@@ -222,6 +222,7 @@ __device__ __forceinline__ void store_split_mirror(__half *base, int64_t pitch, 
 // the diagonal, `blocks_diag` added on the diagonal, a second time
 struct EpiSym
 {
+    static constexpr bool kSquare = true;
     struct Params
     {
         __half *out;
@@ -263,6 +264,7 @@ struct EpiSym
 // X of the next step, in halves
 struct EpiX
 {
+    static constexpr bool kSquare = false;
     struct Params
     {
         __half *out;
@@ -284,6 +286,7 @@ struct EpiX
 // the last step's result: written out, or the parameters' update
 struct EpiOut
 {
+    static constexpr bool kSquare = false;
     struct Params : NsOut
     {
         int64_t ld, stride;
@@ -391,6 +394,7 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
     int rc = arena_begin(2 * a256(batch * x_stride * 2) + 2 * a256(batch * m_stride * 2) + a256(batch * d_stride * 2) + a256(batch * blocks * 8), stream);
     if (rc)
         return rc;
+    const ArenaUse use{stream};
     __half *x[2]    = {static_cast<__half *>(arena_alloc(batch * x_stride * 2)), static_cast<__half *>(arena_alloc(batch * x_stride * 2))};
     __half *A       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
     __half *S       = static_cast<__half *>(arena_alloc(batch * m_stride * 2));
@@ -413,7 +417,7 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
         if ((rc = s16::launch_after(muon_direct_kernel, dim3((unsigned)sblocks, (unsigned)batch), dim3(256), 0, stream, x[0], x_stride, (int)rows, (int)cols, xc,
                                     out)))
             return rc;
-        return arena_end(stream);
+        return kOk;
     }
     GemmArgs gg{};
     gg.batch = (int)batch, gg.splits = 1, gg.err = device_error_flag();
@@ -449,7 +453,7 @@ int orthogonalise(const float *p, float *g, float *buf, const MomentumArgs &a, E
         if (rc)
             return rc;
     }
-    return arena_end(stream);
+    return kOk;
 }
 
 int check_matrix(const char *what, int64_t batch, int64_t rows, int64_t cols, int steps, float eps, int precision)

@@ -278,14 +278,17 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
     // descriptors: K-major with a 128-byte swizzle; X as the reduction's rows, its blocks of 64 columns C::block apart
     auto k_major = [&](int at) { return ptx::make_smem_desc(base + at, 16, 1024, ptx::kLayoutSw128); };
     auto rows_of_x = [&](int at) { return ptx::make_smem_desc(base + at, C::block, 1024, ptx::kLayoutSw128); };
-    // D (+)= hi hi + (lo hi + hi lo first), `n` steps of 16; step k's operands a_step(k), b_step(k) 16-byte units further
+    // D (+)= hi hi + (lo lo + lo hi + hi lo first), `n` steps of 16; step k's operands a_step(k), b_step(k) 16-byte units further.
+    // The accumulator truncates, so it holds 64 of a reduction at most (see gemm_split16.cuh); lo lo is worth its MMA here, where
+    // sums are short: 9 x 14 is 0.9e-6 off instead of 1.3e-6 (plain fp32 products 0.7e-6).
     auto products = [&](uint32_t d, uint64_t a_hi, uint64_t a_lo, uint64_t b_hi, uint64_t b_lo, int n, auto &&a_step, auto &&b_step, uint32_t idesc, uint32_t acc) {
         if (p.terms == 3)
         {
 #pragma unroll 4
             for (int k = 0; k < n; ++k)
             {
-                s16::mma_f16(d, a_lo + a_step(k), b_hi + b_step(k), idesc, acc);
+                s16::mma_f16(d, a_lo + a_step(k), b_lo + b_step(k), idesc, acc);
+                s16::mma_f16(d, a_lo + a_step(k), b_hi + b_step(k), idesc, 1);
                 s16::mma_f16(d, a_hi + a_step(k), b_lo + b_step(k), idesc, 1);
                 acc = 1;
             }
@@ -439,8 +442,12 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
         // A^2 (A is symmetric: both operands K-major), S = a I + b A + c A^2
         if (tid == 0)
         {
-            products(tmem, k_major(o_ahi), k_major(o_alo), k_major(o_ahi), k_major(o_alo), ksq, along_row, along_row,
-                     s16::idesc_f16(128, p.s_pad, false, false), 0);
+            // the reduction's first and second 64 into accumulators of their own
+            for (int k = 0; k < ksq; k += 4)
+            {
+                const uint64_t hi = k_major(o_ahi) + along_row(k), lo = k_major(o_alo) + along_row(k);
+                products(tmem + 32 * k, hi, lo, hi, lo, ksq - k < 4 ? ksq - k : 4, along_row, along_row, s16::idesc_f16(128, p.s_pad, false, false), 0);
+            }
             ptx::mma_commit(bar);
         }
         finish_mmas();
@@ -450,6 +457,15 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
                 uint32_t r[32];
                 ptx::tmem_ld_32x32(lanes + c, r);
                 ptx::tmem_ld_wait();
+                if (RB > 64)
+                {
+                    uint32_t r2[32];
+                    ptx::tmem_ld_32x32(lanes + 128 + c, r2);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
+                }
 #pragma unroll
                 for (int o = 0; o < 32; o += 8)
                 {
@@ -475,17 +491,20 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
             }
         threads_meet();
 
-        // X_loc = S X_loc, 512 columns (TMEM) at a time
-        for (int n0 = 0; n0 < n_loc; n0 += 512)
+        // X_loc = S X_loc, as many columns at a time as TMEM holds (RB = 128: twice, see above)
+        constexpr int kWidth = RB > 64 ? 256 : 512;
+        for (int n0 = 0; n0 < n_loc; n0 += kWidth)
         {
-            const int width = n_loc - n0 < 512 ? n_loc - n0 : 512;
+            const int width = n_loc - n0 < kWidth ? n_loc - n0 : kWidth;
             if (tid == 0)
             {
                 for (int n = 0; n < width; n += 256)
                 {
                     const int cols = width - n < 256 ? width - n : 256, at = (n0 + n) / 64 * C::block;
-                    products(tmem + n, k_major(o_ahi), k_major(o_alo), rows_of_x(at), rows_of_x(o_xlo + at), ksq, along_row, along_rows,
-                             s16::idesc_f16(128, cols, false, true), 0);
+                    for (int k = 0; k < ksq; k += 4)  // (k = 4: RB = 128, n = 0)
+                        products(tmem + n + 64 * k, k_major(o_ahi) + along_row(k), k_major(o_alo) + along_row(k), rows_of_x(at) + along_rows(k),
+                                 rows_of_x(o_xlo + at) + along_rows(k), ksq - k < 4 ? ksq - k : 4, along_row, along_rows,
+                                 s16::idesc_f16(128, cols, false, true), 0);
                 }
                 ptx::mma_commit(bar);
             }
@@ -496,6 +515,15 @@ __global__ void __launch_bounds__(kThreads, 1) muon_small_kernel(const SmallArgs
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(lanes + c, r);
                     ptx::tmem_ld_wait();
+                    if (RB > 64)
+                    {
+                        uint32_t r2[32];
+                        ptx::tmem_ld_32x32(lanes + 256 + c, r2);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
+                    }
                     if (row < RB)
                     {
 #pragma unroll
