@@ -9,6 +9,7 @@
 //   X_loc = S X_loc                (the same X_loc read MN-major)
 // A product of 128 x 128 takes under a microsecond here, so the steps' latencies (commit, TMEM reads, two cluster barriers)
 // bound the kernel; the form of three GEMM launches per step pays set-up, ring fill and global stores 3 * steps times instead.
+// 128 x 128: 59 us for five steps (the chain of launches 122), 32 of 64 x 512 52 us (116), 15 of 5 x 5888 92 us (414).
 // The waits on the tensor core are bounded; one that gives up raises the error flag and the kernel runs on to its end (the cluster
 // barriers need every CTA).
 #include <cuda_runtime.h>

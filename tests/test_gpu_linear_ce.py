@@ -338,6 +338,26 @@ def test_captured_and_replayed(ops):
         assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 5000, 100), (40, 5000, 128), (200, 900, 64)])
+def test_loss_alone_captured_and_on_another_stream(ops, M, N, K):
+    x, w, t, b = make(M, N, K, seed=40, bias=True)
+    run = lambda: ops.linear_cross_entropy(x, w, t, b=b, need_dx=False, need_dw=False, need_db=False)[:2]  # noqa: E731
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        again = run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = run()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, c, d in zip(want, again, out):
+        assert torch.equal(a, c) and torch.equal(a, d)
+
+
 def test_unaligned_tensors(ops):
     """Every buffer starts 4 bytes off a 16-byte boundary."""
     off = lambda v: torch.empty(v.numel() + 1, device="cuda", dtype=v.dtype)[1:].view(v.shape).copy_(v)  # noqa: E731

@@ -228,8 +228,9 @@ def test_same_bits_again_and_on_other_streams(ops):
         assert torch.equal(ga, wa) and torch.equal(gc, wc)
 
 
-def test_captured_and_replayed(ops):
-    p, g, buf = (gradient(150, 260, seed=s) for s in (1, 2, 3))
+@pytest.mark.parametrize("shape", [(150, 260), (40, 300), (3, 100, 700), (2, 300, 140)])
+def test_captured_and_replayed(ops, shape):
+    p, g, buf = (gradient(*shape, seed=s) for s in (1, 2, 3))
     start = [v.clone() for v in (p, buf)]
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):
